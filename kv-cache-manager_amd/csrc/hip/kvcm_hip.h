@@ -155,6 +155,27 @@ int kvcm_attention_prefill(const void* q, int q_stride, void* out, int out_strid
                            int max_run, int T, int max_context, int nh, int nkv, int hd, int B, float scale,
                            float* scratch, long long scratch_floats, const float* cos_sin, hipStream_t s);
 
+// ---- the cache held in 4 bits (cache4.h has its format; uint8 [pages][nkv][page / 16][16 * (hd + 8)]) -------------------
+// hd 32, 64, 128 or 256; pages of a multiple of 16 tokens.
+int kvcm_cache4_supported(int nh, int nkv, int hd, int page);
+// Rows [q | k | v] of T tokens: q and k rotated by cos_sin [T][hd / 2] (null: not rotated, q not touched), q to q_out (which may
+// be the rows' own), k and v to their slots (a slot outside the pages: kept nowhere).
+int kvcm_rope_cache4(const void* qkv, int dtype, int stride, void* q_out, int q_stride, void* cache, const int* slots, const void* cos_sin, int T, int nh,
+                     int nkv, int hd, int pages, int page, hipStream_t stream);
+// The tokens at n slots as rows [nkv * hd] of keys and of values (zeros for a slot outside the pages).
+int kvcm_cache4_rows(const void* cache, const int* slots, void* k, int k_stride, void* v, int v_stride, int dtype, int n, int nkv, int hd, int pages, int page,
+                     hipStream_t stream);
+// Attention over it: for T rows of different sequences (row_seq, ctx_lens), and for runs of rows as kvcm_attention_prefill has
+// them.  window > 0: a row sees the last `window` tokens of its context.  Scratch floats by the _scratch entries.
+long long kvcm_attention_decode4_scratch(int T, int nh, int nkv, int hd, int max_context, int window);
+int kvcm_attention_decode4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride, int seqs,
+                           const int* row_seq, const int* ctx_lens, int T, int nh, int nkv, int hd, int pages, int page, float scale, int window, int max_context,
+                           float* scratch, long long scratch_floats, hipStream_t stream);
+long long kvcm_attention_prefill4_scratch(int T, int nh, int nkv, int hd, int max_context, int max_run, int num_seqs, int window);
+int kvcm_attention_prefill4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride,
+                            const int* run_start, const int* seq_start, int num_seqs, int max_run, int T, int nh, int nkv, int hd, int pages, int page, float scale,
+                            int window, int max_context, float* scratch, long long scratch_floats, hipStream_t stream);
+
 // ---- sampling ---------------------------------------------------------------------------------
 int kvcm_sample(const float* logits, int ld, const float* temperature, const uint64_t* seeds, const long long* request_ids,
                 const int* token_index, int* out, int R, int V, hipStream_t s);

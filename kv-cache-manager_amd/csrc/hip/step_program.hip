@@ -98,6 +98,10 @@ const Entry kEntries[] = {
     KVCM_ENTRY(kvcm_attention_decode),
     KVCM_ENTRY(kvcm_attention_decode_fused),
     KVCM_ENTRY(kvcm_attention_prefill),
+    KVCM_ENTRY(kvcm_rope_cache4),
+    KVCM_ENTRY(kvcm_cache4_rows),
+    KVCM_ENTRY(kvcm_attention_decode4),
+    KVCM_ENTRY(kvcm_attention_prefill4),
     KVCM_ENTRY(kvcm_sample),
     KVCM_ENTRY(kvcm_embed_scaled),
     KVCM_ENTRY(kvcm_gated_act),

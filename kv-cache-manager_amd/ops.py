@@ -90,6 +90,14 @@ def _declare(lib):
     lib.kvcm_attention_decode_scratch.restype = C.c_longlong
     lib.kvcm_attention_decode_scratch.argtypes = [i, i, i, i]
     fn("kvcm_attention_decode", vp, i, vp, i, vp, vp, vp, i, vp, vp, i, i, i, i, i, f, i, vp, C.c_longlong, vp)
+    fn("kvcm_cache4_supported", i, i, i, i)
+    fn("kvcm_rope_cache4", vp, i, i, vp, i, vp, vp, vp, i, i, i, i, i, i, vp)
+    fn("kvcm_cache4_rows", vp, vp, vp, i, vp, i, i, i, i, i, i, i, vp)
+    for name, n in (("decode", 6), ("prefill", 8)):
+        scratch = getattr(lib, f"kvcm_attention_{name}4_scratch")
+        scratch.restype, scratch.argtypes = C.c_longlong, [i] * n
+    fn("kvcm_attention_decode4", vp, i, i, vp, i, vp, vp, i, i, vp, vp, i, i, i, i, i, i, f, i, i, vp, C.c_longlong, vp)
+    fn("kvcm_attention_prefill4", vp, i, i, vp, i, vp, vp, i, vp, vp, i, i, i, i, i, i, i, i, f, i, i, vp, C.c_longlong, vp)
     fn("kvcm_gemm_library", vp, vp, vp, i, i, i, i, i, i, vp, C.c_longlong, vp)
     fn("kvcm_gemm_library_tuned", i, i, i, i, i, i)
     fn("kvcm_gemm_library_f32out_plan", i, i, i, i, i, i)
@@ -1200,6 +1208,142 @@ def attention_prefill(q, out, kcache, vcache, tables, table_stride, run_start, s
                                         _ptr(tables), table_stride, _ptr(run_start), _ptr(seq_start), num_seqs, max_run,
                                         T, int(max_context), nh, nkv, hd, kcache.shape[2], float(scale), _ptr(scratch),
                                         scratch.numel() if scratch is not None else 0, _ptr(cos_sin), _stream())
+
+
+# ------------------------------------------------------------------------- the cache held in 4 bits
+def cache4_supported(nh, nkv, hd, dtype, block_size=16):
+    """Whether the operators below take these sizes: head_dim 32, 64, 128 or 256, pages of a multiple of 16 tokens, rows of bfloat16
+    or float32."""
+    return dtype in _DT and bool(lib().kvcm_cache4_supported(nh, nkv, hd, block_size))
+
+
+def cache4_shape(pages, nkv, hd, block_size=16):
+    """The shape of a 4-bit cache, a uint8 tensor: tiles of 16 tokens of one kv head, ``hd`` + 8 bytes a token for its key and its value.
+    Each of the two is kept as 4-bit codes between its own smallest and largest entry: value = low + step * code, with low and step in
+    bfloat16 and step a fifteenth of the range, so that an entry is off by about half a step at most.  A vector that holds an Inf or a
+    NaN reads as NaN."""
+    _need(pages > 0 and nkv > 0 and hd in (32, 64, 128, 256) and block_size > 0 and block_size % 16 == 0,
+          "a 4-bit cache has pages of a multiple of 16 tokens and head_dim 32, 64, 128 or 256")
+    return (pages, nkv, block_size // 16, 16 * (hd + 8))
+
+
+def _one_gpu(*ts):
+    """Launches go to device 0's current stream: every operand lives there, and it is the current device."""
+    _dev(*ts)
+    for t in ts:
+        _need(t is None or t.get_device() == 0, "kernel operands must live on device 0")
+    _need(torch.cuda.current_device() == 0, "device 0 must be the current device")
+
+
+def _check_cache4(cache, nkv, hd, nh=None):
+    _need(cache.dtype == torch.uint8 and cache.dim() == 4 and cache.is_contiguous() and cache.data_ptr() % 16 == 0
+          and tuple(cache.shape) == cache4_shape(cache.shape[0], nkv, hd, 16 * cache.shape[2]),
+          "the cache must be contiguous uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)], aligned to 16 bytes (cache4_shape)")
+    _need(cache.shape[0] * cache.shape[2] * 16 < 2 ** 31, "a cache of 2^31 token slots or more does not fit 32-bit slot numbers")
+    _need(nh is None or (nh > 0 and nh % nkv == 0), "the heads must be a multiple of the kv heads")
+    return cache.shape[0], 16 * cache.shape[2]
+
+
+def _long_rows(t, name, rows, cols, dtype=None):
+    _rows2d(t, name)
+    _need(t.dtype in _DT and (dtype is None or t.dtype == dtype), f"{name} must be {'bfloat16 or float32' if dtype is None else dtype}")
+    _need(t.shape[0] >= rows >= 0 and t.shape[1] >= cols and (t.stride(0) >= cols or rows <= 1) and t.stride(0) < 2 ** 31,
+          f"{name} must be [>= {rows}, >= {cols}] with rows of their own")
+    return max(t.stride(0), cols)      # (a single row's stride may be anything)
+
+
+def rope_cache4(qkv, nh, nkv, hd, cache, slots, cos_sin=None, q_out=None, rows=None):
+    """Writes the k and v heads of the fused rows [q | k | v] to the slots (page * block_size + place, each at most once; one
+    outside the pages, such as -1: kept nowhere) of a 4-bit cache (``cache4_shape``).  With a table of angles ``cos_sin`` (float32
+    [rows, hd/2, 2]) k is rotated before, as ``rope_cache`` does, and q as well, to ``q_out`` [rows, nh * hd] (default: in its place
+    in ``qkv``); k and v of ``qkv`` stay as they are.  Without it nothing is rotated and q is not touched."""
+    T = qkv.shape[0] if rows is None else rows
+    _one_gpu(qkv, cache, slots, cos_sin, q_out)
+    pages, page = _check_cache4(cache, nkv, hd, nh)
+    stride = _long_rows(qkv, "qkv", T, (nh + 2 * nkv) * hd)
+    _i32(slots, "slots", T)
+    _need(cos_sin is not None or q_out is None, "q_out is for rotated queries: cos_sin is missing")
+    q_stride = 0
+    if cos_sin is not None:
+        _need(cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.numel() >= T * hd and cos_sin.data_ptr() % 16 == 0,
+              "cos_sin must be float32 [rows, head_dim/2, 2], aligned to 16 bytes")
+        q_out = qkv if q_out is None else q_out
+        q_stride = _long_rows(q_out, "q_out", T, nh * hd, qkv.dtype)
+    _call("kvcm_rope_cache4", _ptr(qkv), _DT[qkv.dtype], stride, _ptr(q_out), q_stride, _ptr(cache), _ptr(slots), _ptr(cos_sin), T, nh, nkv, hd,
+          pages, page, _stream())
+
+
+def cache4_rows(cache, slots, k, v, rows=None):
+    """Reads the tokens at ``slots`` back from a 4-bit cache: k, v [rows, nkv * hd] (bfloat16 or float32, both alike).  A slot outside the
+    pages (-1) gives zeros."""
+    n = slots.numel() if rows is None else rows
+    _one_gpu(cache, slots, k, v)
+    _need(cache.dim() == 4, "the cache must be uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)] (cache4_shape)")
+    nkv, hd = cache.shape[1], cache.shape[3] // 16 - 8
+    pages, page = _check_cache4(cache, nkv, hd)
+    _i32(slots, "slots", n)
+    k_stride, v_stride = _long_rows(k, "k", n, nkv * hd), _long_rows(v, "v", n, nkv * hd, k.dtype)
+    _call("kvcm_cache4_rows", _ptr(cache), _ptr(slots), _ptr(k), k_stride, _ptr(v), v_stride, _DT[k.dtype], n, nkv, hd, pages, page, _stream())
+
+
+def _scratch4(what, need, scratch, device):
+    if need and scratch is None:
+        _need(_recording is None, f"{what}: a recorded step must bring its scratch (an allocation here would not outlive the step)")
+        scratch = torch.empty(need, dtype=torch.float32, device=device)
+    _need(scratch is None or (scratch.dtype == torch.float32 and scratch.is_contiguous()), "scratch must be contiguous float32")
+    _need(scratch is None or scratch.numel() >= need, f"{what}: scratch of {need} floats is needed")
+    return scratch
+
+
+def attention_decode4_scratch(rows, nh, nkv, hd, max_context, window=0):
+    """Floats of scratch ``attention_decode4`` needs for these sizes (0: contexts are not cut)."""
+    return int(lib().kvcm_attention_decode4_scratch(rows, nh, nkv, hd, int(max_context), int(window)))
+
+
+def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh, nkv, hd, scale, max_context, scratch=None, window=0, rows=None):
+    """``attention`` over a 4-bit cache for rows of different sequences (bfloat16 or float32): out[r, h] = softmax(scale * q[r, h] . K) V
+    over the tokens 0 .. ctx_lens[r] - 1 of sequence row_seq[r] (``window`` > 0: the last ``window`` of them).  A row that sees nothing (a
+    context of 0, a sequence without a table) gives zeros, and so would one whose pages all lie outside the cache: a table's entry that is
+    no page hides its tokens.  ``max_context`` bounds every row's context length and decides how contexts are cut into parts that run side
+    by side, which needs ``scratch`` (attention_decode4_scratch floats; allocated here when not given)."""
+    T = q.shape[0] if rows is None else rows
+    _one_gpu(q, out, cache, tables, row_seq, ctx_lens, scratch)
+    pages, page = _check_cache4(cache, nkv, hd, nh)
+    q_stride, out_stride = _long_rows(q, "q", T, nh * hd), _long_rows(out, "out", T, nh * hd, q.dtype)
+    for t, name, n in ((row_seq, "row_seq", T), (ctx_lens, "ctx_lens", T), (tables, "tables", 1)):
+        _i32(t, name, n)
+    _need(table_stride > 0 and tables.numel() >= table_stride, "tables must hold rows of table_stride pages")
+    _need(window >= 0 and max_context >= 0, "window and max_context must not be negative")
+    scratch = _scratch4("attention_decode4", attention_decode4_scratch(T, nh, nkv, hd, max_context, window), scratch, q.device)
+    _call("kvcm_attention_decode4", _ptr(q), _DT[q.dtype], q_stride, _ptr(out), out_stride, _ptr(cache), _ptr(tables), table_stride,
+          tables.numel() // table_stride, _ptr(row_seq), _ptr(ctx_lens), T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context),
+          _ptr(scratch), scratch.numel() if scratch is not None else 0, _stream())
+
+
+def attention_prefill4_scratch(rows, nh, nkv, hd, max_context, max_run, num_seqs, window=0):
+    """Floats of scratch ``attention_prefill4`` needs for a launch of these sizes (0: contexts are not cut)."""
+    return int(lib().kvcm_attention_prefill4_scratch(rows, nh, nkv, hd, int(max_context), max_run, num_seqs, int(window)))
+
+
+def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start, num_seqs, max_run, nh, nkv, hd, scale, rows=None,
+                       max_context=None, scratch=None, window=0):
+    """Causal attention over a 4-bit cache for runs of consecutive positions, as ``attention_prefill`` has them: sequence s owns rows
+    run_start[s] .. run_start[s+1]-1, at most ``max_run``, the first of them at position seq_start[s]; every row sees the sequence's cached
+    tokens up to its own position (``window`` > 0: the last ``window`` of them).  Rows of no run are left as they are.
+    ``max_context``: a bound of every row's context length (default: what the tables can hold)."""
+    T = q.shape[0] if rows is None else rows
+    _one_gpu(q, out, cache, tables, run_start, seq_start, scratch)
+    pages, page = _check_cache4(cache, nkv, hd, nh)
+    q_stride, out_stride = _long_rows(q, "q", T, nh * hd), _long_rows(out, "out", T, nh * hd, q.dtype)
+    _need(table_stride > 0 and num_seqs >= 0 and max_run >= 0 and window >= 0, "table_stride must be positive, num_seqs, max_run and window not negative")
+    for t, name, n in ((run_start, "run_start", num_seqs + 1), (seq_start, "seq_start", num_seqs), (tables, "tables", num_seqs * table_stride)):
+        _i32(t, name, n)
+    max_context = table_stride * page if max_context is None else max_context
+    _need(max_context >= 0, "max_context must not be negative")
+    scratch = _scratch4("attention_prefill4", attention_prefill4_scratch(T, nh, nkv, hd, max_context, max_run, num_seqs, window), scratch, q.device)
+    _call("kvcm_attention_prefill4", _ptr(q), _DT[q.dtype], q_stride, _ptr(out), out_stride, _ptr(cache), _ptr(tables), table_stride, _ptr(run_start),
+          _ptr(seq_start), num_seqs, max_run, T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context), _ptr(scratch),
+          scratch.numel() if scratch is not None else 0, _stream())
 
 
 # ------------------------------------------------------------------------- probes of the machine

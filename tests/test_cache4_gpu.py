@@ -1,0 +1,329 @@
+"""The operators of the 4-bit cache on the GPU against plain ones in 64 bits (plain_cache4.py)."""
+import numpy as np
+import pytest
+import torch
+
+import plain_cache4 as plain
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from kvcm_amd import ops as _ops
+    _ops.lib()
+    return _ops
+
+
+def ints(v):
+    return torch.tensor(list(v), dtype=torch.int32, device=DEV)
+
+
+def garbage(ops, pages, nkv, hd, page, gen):
+    """A cache whose every byte is anything: what reused pages hold beyond their owner's tokens (NaN and Inf steps among it)."""
+    return torch.randint(0, 256, ops.cache4_shape(pages, nkv, hd, page), generator=gen, dtype=torch.uint8).to(DEV)
+
+
+def filled(ops, pages, nkv, hd, page, gen, slots, dtype=BF):
+    """Garbage, with sound tokens at ``slots``."""
+    cache = garbage(ops, pages, nkv, hd, page, gen)
+    x = torch.randn(len(slots), 3 * nkv * hd, generator=gen) + 2 * (torch.rand(3 * nkv * hd, generator=gen) < 0.1)
+    ops.rope_cache4(x.to(dtype).to(DEV), nkv, nkv, hd, cache, ints(slots))
+    return cache
+
+
+# ----------------------------------------------------------------------------------- writing and reading
+def rotated(x, cos_sin, dtype):
+    """[rows, heads, hd] rotated as the rows' type has it: bfloat16 in 32 bits (one product rounded, the other kept whole), float32 in 64."""
+    a, b = np.split(x, 2, -1)
+    cs, sn = (cos_sin[:, None, :, i].astype(np.float64) for i in (0, 1))
+    if dtype == F32:
+        return np.concatenate([(a * cs - b * sn).astype(np.float32), (b * cs + a * sn).astype(np.float32)], -1).astype(np.float64)
+    r32 = lambda v: v.astype(np.float32).astype(np.float64)
+    return plain.bf16(np.concatenate([r32(a * cs - r32(b * sn)), r32(b * cs + r32(a * sn))], -1))
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+@pytest.mark.parametrize("nh, nkv, hd, page, rotate", ((3, 1, 32, 16, True), (8, 2, 64, 32, True), (4, 4, 128, 16, True), (2, 1, 256, 48, True), (8, 2, 64, 16, False),
+                                                       (2, 2, 32, 64, False)))
+def test_store_writes_the_format_and_nothing_else(ops, nh, nkv, hd, page, rotate, dtype):
+    gen = torch.Generator().manual_seed(nh * hd + page)
+    T, pages, width = 23, 7, (nh + 2 * nkv) * hd
+    rows = torch.randn(T, width, generator=gen) * torch.exp(2 * torch.randn(T, 1, generator=gen))
+    rows[3] = 0.0
+    rows[4] = 1.5                                        # no range: step 0
+    rows[5, ::3] = 2.0 ** -130                           # ranges of denormal steps
+    rows[6] *= 1e30
+    if not rotate:
+        rows[7, nh * hd + 1] = float("inf")
+        rows[8, -1] = float("nan")
+        rows[9, -hd:] = float("-inf")
+        rows[10, nh * hd] = -3.3e38
+        rows[11, nh * hd] = 3e-39
+    wide = torch.full((T, width + 24), 7.0).to(dtype)
+    wide[:, 8:8 + width] = rows.to(dtype)
+    held = wide.to(DEV)
+    qkv = held[:, 8:8 + width] if dtype == F32 else held[:, 8:8 + width]
+    slots = torch.randperm(pages * page, generator=gen)[:T].tolist()
+    slots[12], slots[13], slots[14] = -1, pages * page, -2 ** 31
+    before = garbage(ops, pages, nkv, hd, page, gen)
+    cache = before.clone()
+    table = None
+    if rotate:
+        angles = torch.rand(T, hd // 2, generator=gen) * 40
+        table = torch.stack([angles.cos(), angles.sin()], -1).contiguous()
+    ops.rope_cache4(qkv, nh, nkv, hd, cache, ints(slots), cos_sin=None if table is None else table.to(DEV))
+    x = rows.to(dtype).double().numpy().reshape(T, nh + 2 * nkv, hd)
+    if rotate:
+        x[:, :nh + nkv] = rotated(x[:, :nh + nkv], table.numpy(), dtype)
+    want = before.cpu().numpy()
+    for r, s in enumerate(slots):
+        if 0 <= s < pages * page:
+            for g in range(nkv):
+                plain.write(want, s, g, x[r, nh + g], x[r, nh + nkv + g])
+    np.testing.assert_array_equal(cache.cpu().numpy(), want)
+    after = held.cpu()
+    assert torch.equal(after[:, :8], wide[:, :8]) and torch.equal(after[:, 8 + width:], wide[:, 8 + width:])
+    assert torch.equal(after[:, 8 + nh * hd:8 + width].nan_to_num(5.0), wide[:, 8 + nh * hd:8 + width].nan_to_num(5.0))
+    assert torch.equal(after[:, 8:8 + nh * hd].double(), torch.as_tensor(x[:, :nh]).reshape(T, -1))
+
+
+def test_store_takes_one_row_many_rows_none_and_a_place_for_the_queries(ops):
+    gen = torch.Generator().manual_seed(5)
+    nh, nkv, hd, page, pages = 4, 2, 64, 16, 90
+    for T in (0, 1, 1300):
+        qkv = torch.randn(max(T, 2), (nh + 2 * nkv) * hd, generator=gen).to(BF).to(DEV)
+        angles = torch.rand(max(T, 2), hd // 2, generator=gen)
+        table = torch.stack([angles.cos(), angles.sin()], -1).to(DEV)
+        slots = torch.randperm(pages * page, generator=gen)[:max(T, 2)].to(torch.int32).to(DEV)
+        one, two = (torch.zeros(ops.cache4_shape(pages, nkv, hd, page), dtype=torch.uint8, device=DEV) for _ in range(2))
+        kept, q = qkv.clone(), torch.full((max(T, 2), nh * hd + 3), 9.0, dtype=BF, device=DEV)
+        ops.rope_cache4(qkv, nh, nkv, hd, one, slots, cos_sin=table, q_out=q, rows=T)
+        assert torch.equal(qkv, kept)
+        ops.rope_cache4(qkv, nh, nkv, hd, two, slots, cos_sin=table, rows=T)
+        assert torch.equal(one, two) and torch.equal(q[:T, :nh * hd], qkv[:T, :nh * hd]) and torch.equal(qkv[T:], kept[T:])
+        assert bool((q[:, nh * hd:] == 9).all()) and bool((q[T:] == 9).all())
+        assert T > 0 or not one.any()
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+@pytest.mark.parametrize("nkv, hd, page", ((1, 32, 16), (3, 64, 32), (2, 128, 16), (2, 256, 16)))
+def test_read_gives_what_the_bytes_stand_for(ops, nkv, hd, page, dtype):
+    gen = torch.Generator().manual_seed(hd)
+    pages = 5
+    slots = list(range(pages * page))
+    cache = filled(ops, pages, nkv, hd, page, gen, slots)
+    order = torch.randperm(len(slots), generator=gen)[:57].tolist() + [-1, pages * page, 3, 3]      # one twice, two of none
+    k, v = (torch.full((len(order) + 1, nkv * hd + 5), 9.0, dtype=dtype, device=DEV) for _ in range(2))
+    ops.cache4_rows(cache, ints(order), k, v)
+    kc, ks, kl, vc, vs, vl = plain.parts(cache, nkv, hd)
+    valid = torch.tensor([0 <= s < pages * page for s in order], device=DEV)
+    at = ints(order).long().clamp(0, pages * page - 1)
+    for got, want in ((k, kl + ks * kc), (v, vl + vs * vc)):
+        want = torch.where(valid.view(-1, 1), want[at].flatten(1), torch.zeros((), dtype=torch.float64, device=DEV))
+        assert torch.equal(got[:-1, :nkv * hd], want.to(dtype))
+        assert bool((got[:, nkv * hd:] == 9).all()) and bool((got[-1] == 9).all())
+
+
+def test_a_token_is_within_half_a_step(ops):
+    """|x - value| <= step / 2 + 15 * 2^-9 step at the top (a step rounded down) for bfloat16 vectors, whose low is exact."""
+    gen = torch.Generator().manual_seed(2)
+    nkv, hd, T = 4, 128, 256
+    x = torch.randn(T, 3 * nkv * hd, generator=gen).to(BF).to(DEV)
+    cache = torch.zeros(ops.cache4_shape(16, nkv, hd, 16), dtype=torch.uint8, device=DEV)
+    ops.rope_cache4(x, nkv, nkv, hd, cache, ints(range(T)))
+    k, v = (torch.empty(T, nkv * hd, device=DEV) for _ in range(2))
+    ops.cache4_rows(cache, ints(range(T)), k, v)
+    for got, want in ((k, x[:, nkv * hd:2 * nkv * hd]), (v, x[:, 2 * nkv * hd:])):
+        a, b = got.view(T, nkv, hd), want.float().view(T, nkv, hd)
+        step = (b.amax(-1, keepdim=True) - b.amin(-1, keepdim=True)) / 15
+        assert bool(((a - b).abs() <= step * (0.5 * (1 + 2.0 ** -8) + 15 * 2.0 ** -9 + 1e-5)).all())
+
+
+# ----------------------------------------------------------------------------------- attention
+SIZES = ((4, 4, 32, 16), (8, 1, 64, 16), (6, 2, 64, 32), (8, 8, 128, 16), (8, 2, 128, 64), (34, 2, 64, 16), (4, 2, 256, 16))
+
+
+class Sequences:
+    """Page tables of sequences of given lengths over a shuffled pool with garbage in every other place."""
+
+    def __init__(self, ops, nh, nkv, hd, page, lengths, gen, dtype, spare=2):
+        self.nh, self.nkv, self.hd, self.page, self.dtype = nh, nkv, hd, page, dtype
+        need = [-(-n // page) for n in lengths]
+        self.pages, self.stride = sum(need) + spare, max(max(need), 1) + 1
+        order = torch.randperm(self.pages, generator=gen).tolist()
+        self.tables = torch.randint(-2 ** 31, 2 ** 31 - 1, (len(lengths), self.stride), generator=gen).to(torch.int32)      # beyond a length: anything
+        self.slots = []
+        for i, n in enumerate(lengths):
+            mine = [order.pop() for _ in range(need[i])]
+            self.tables[i, :len(mine)] = torch.tensor(mine, dtype=torch.int32)
+            self.slots.append(torch.tensor([mine[t // page] * page + t % page for t in range(n)], dtype=torch.long, device=DEV))
+        self.cache = filled(ops, self.pages, nkv, hd, page, gen, torch.cat(self.slots).tolist(), dtype)
+        self.held = plain.parts(self.cache, nkv, hd)
+        self.dev_tables = self.tables.to(DEV).view(-1)
+
+    def expect(self, q, seqs, visible, scale):
+        none = torch.zeros(0, dtype=torch.long, device=DEV)
+        return plain.attend(q.double().view(q.shape[0], self.nh, self.hd), self.held, [self.slots[s] if s >= 0 else none for s in seqs], visible,
+                            self.nh, self.nkv, scale, self.dtype)
+
+
+def near(out, want, tol):
+    got = out.double().view(want.shape)
+    assert not bool(got.isnan().any())
+    worst = ((got - want).abs() / tol.clamp_min(1e-30)).max()
+    assert bool(((got - want).abs() <= tol).all()), f"{float(worst):.3f} of the tolerance"
+
+
+def queries(rows, width, dtype, gen, extra=0):
+    return torch.randn(rows, width + extra, generator=gen).to(dtype).to(DEV)
+
+
+LENGTHS = (1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 300)
+
+
+@pytest.mark.parametrize("window", (0, 1, 40))
+@pytest.mark.parametrize("dtype", (BF, F32))
+@pytest.mark.parametrize("nh, nkv, hd, page", SIZES)
+def test_decode(ops, nh, nkv, hd, page, dtype, window):
+    gen = torch.Generator().manual_seed(nh * hd + page)
+    s = Sequences(ops, nh, nkv, hd, page, LENGTHS, gen, dtype)
+    # every sequence twice, the second time not to its end; padding rows between; sequences that have no table
+    seqs = list(range(len(LENGTHS))) + list(range(len(LENGTHS))) + [0, 3, -1, len(LENGTHS)]
+    ctx = list(LENGTHS) + [max(1, n // 2) for n in LENGTHS] + [0, -7, 20, 20]
+    order = torch.randperm(len(seqs), generator=gen).tolist()
+    seqs, ctx = [seqs[i] for i in order], [ctx[i] for i in order]
+    T = len(seqs)
+    q = queries(T + 2, nh * hd, dtype, gen, extra=2 * nkv * hd)
+    out = torch.full((T + 2, nh * hd + 8), 9.0, dtype=dtype, device=DEV)
+    scale = hd ** -0.5
+    ops.attention_decode4(q, out, s.cache, s.dev_tables, s.stride, ints(seqs), ints(ctx), nh, nkv, hd, scale, max(LENGTHS), window=window, rows=T)
+    sound = [0 <= n < len(LENGTHS) for n in seqs]
+    visible = [(max(0, c - window) if window else 0, c) if ok else (0, 0) for c, ok in zip(ctx, sound)]
+    want, tol = s.expect(q[:T, :nh * hd], [n if ok else -1 for n, ok in zip(seqs, sound)], visible, scale)
+    near(out[:T, :nh * hd], want, tol)
+    assert bool((out[:, nh * hd:] == 9).all()) and bool((out[T:] == 9).all())
+
+
+@pytest.mark.parametrize("rows, ctx, window", ((1, 5000, 0), (3, 4097, 0), (1, 5000, 4000), (2, 1500, 0), (40, 700, 0)))
+@pytest.mark.parametrize("nh, nkv, hd, dtype", ((8, 1, 64, BF), (4, 2, 128, BF), (4, 2, 64, F32)))
+def test_decode_over_contexts_cut_into_parts(ops, nh, nkv, hd, dtype, rows, ctx, window):
+    gen = torch.Generator().manual_seed(rows + ctx)
+    lengths = [ctx] + [max(1, ctx // (i + 1) - i) for i in range(1, rows)]
+    s = Sequences(ops, nh, nkv, hd, 16, lengths, gen, dtype)
+    q, out = queries(rows, nh * hd, dtype, gen), torch.empty(rows, nh * hd, dtype=dtype, device=DEV)
+    args = (q, out, s.cache, s.dev_tables, s.stride, ints(range(rows)), ints(lengths), nh, nkv, hd, hd ** -0.5)
+    visible = [(max(0, n - window) if window else 0, n) for n in lengths]
+    want, tol = s.expect(q, range(rows), visible, hd ** -0.5)
+    for bound in (ctx, 4 * ctx):
+        ops.attention_decode4(*args, bound, window=window)
+        near(out, want, tol)
+    first = out.clone()
+    ops.attention_decode4(*args, 4 * ctx, window=window)
+    assert torch.equal(first, out)
+
+
+@pytest.mark.parametrize("window", (0, 1, 29))
+@pytest.mark.parametrize("dtype", (BF, F32))
+@pytest.mark.parametrize("nh, nkv, hd, page", SIZES)
+def test_prefill(ops, nh, nkv, hd, page, dtype, window):
+    gen = torch.Generator().manual_seed(nh + hd + page)
+    runs = (1, 70, 2, 0, 17, 33, 1, 16, 5)
+    starts = (0, 0, 15, 7, 16, 100, 63, 1, 290)
+    s = Sequences(ops, nh, nkv, hd, page, [r + p for r, p in zip(runs, starts)], gen, dtype)
+    first = np.concatenate([[3], 3 + np.cumsum(runs)])      # rows before the first run and behind the last belong to nobody
+    T = int(first[-1]) + 4
+    q = queries(T, nh * hd, dtype, gen, extra=2 * nkv * hd)
+    out = torch.full((T, nh * hd), 9.0, dtype=dtype, device=DEV)
+    scale = hd ** -0.5
+    ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints(first), ints(starts), len(runs), max(runs), nh, nkv, hd, scale, window=window)
+    seqs = [i for i, r in enumerate(runs) for _ in range(r)]
+    pos = [p + j for r, p in zip(runs, starts) for j in range(r)]
+    want, tol = s.expect(q[3:T - 4, :nh * hd], seqs, [(max(0, p + 1 - window) if window else 0, p + 1) for p in pos], scale)
+    near(out[3:T - 4], want, tol)
+    assert bool((out[:3] == 9).all()) and bool((out[T - 4:] == 9).all())
+
+
+@pytest.mark.parametrize("runs, starts, window", (((3,), (3000,), 0), ((130, 40), (900, 2100), 0), ((100,), (2000,), 1500), ((257,), (0,), 0)))
+@pytest.mark.parametrize("nh, nkv, hd, dtype", ((8, 1, 64, BF), (2, 2, 128, BF), (4, 2, 64, F32)))
+def test_prefill_behind_long_contexts(ops, nh, nkv, hd, dtype, runs, starts, window):
+    gen = torch.Generator().manual_seed(sum(starts))
+    s = Sequences(ops, nh, nkv, hd, 16, [r + p for r, p in zip(runs, starts)], gen, dtype)
+    first = np.concatenate([[0], np.cumsum(runs)])
+    T = int(first[-1])
+    q, out = queries(T, nh * hd, dtype, gen), torch.empty(T, nh * hd, dtype=dtype, device=DEV)
+    args = (q, out, s.cache, s.dev_tables, s.stride, ints(first), ints(starts), len(runs), max(runs), nh, nkv, hd, hd ** -0.5)
+    seqs = [i for i, r in enumerate(runs) for _ in range(r)]
+    pos = [p + j for r, p in zip(runs, starts) for j in range(r)]
+    rows = list(range(0, T, 7)) + [T - 1]
+    want, tol = s.expect(q[rows], [seqs[i] for i in rows], [(max(0, pos[i] + 1 - window) if window else 0, pos[i] + 1) for i in rows], hd ** -0.5)
+    for kw in (dict(max_context=max(r + p for r, p in zip(runs, starts))), {}):
+        ops.attention_prefill4(*args, window=window, **kw)
+        near(out[rows], want, tol)
+    again = out.clone()
+    ops.attention_prefill4(*args, window=window)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+def test_infinities_and_nan_stay_with_the_rows_that_see_them(ops, dtype):
+    """A token whose key (or value) is not finite: rows before it, rows of other heads and rows whose window has passed it are as ever."""
+    nh, nkv, hd, page, n, bad = 4, 2, 64, 16, 90, 50
+    gen = torch.Generator().manual_seed(1)
+    s = Sequences(ops, nh, nkv, hd, page, (n,), gen, dtype)
+    rows = torch.randn(2, 3 * nkv * hd, generator=gen).to(dtype)
+    rows[0, nkv * hd + 5] = float("nan")          # token 50: the first kv head's key
+    rows[1, -1] = float("inf")                    # token 51: the second's value
+    ops.rope_cache4(rows.to(DEV), nkv, nkv, hd, s.cache, s.slots[0][bad:bad + 2].to(torch.int32))
+    s.held = plain.parts(s.cache, nkv, hd)
+    q = queries(n, nh * hd, dtype, gen)
+    scale, window = hd ** -0.5, 20
+    for w in (0, window):
+        out, one = torch.empty(n, nh * hd, dtype=dtype, device=DEV), torch.empty(n, nh * hd, dtype=dtype, device=DEV)
+        ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints([0, n]), ints([0]), 1, n, nh, nkv, hd, scale, window=w)
+        ops.attention_decode4(q, one, s.cache, s.dev_tables, s.stride, ints([0] * n), ints(range(1, n + 1)), nh, nkv, hd, scale, n, window=w)
+        want, tol = s.expect(q, [0] * n, [(max(0, p + 1 - w) if w else 0, p + 1) for p in range(n)], scale)
+        for got in (out, one):
+            got = got.double().view(n, nh, hd)
+            for g in range(nkv):
+                mine = torch.arange(n, device=DEV)
+                sees = (mine >= bad + g) & ((mine - w < bad + g) if w else True)
+                of = slice(g * nh // nkv, (g + 1) * nh // nkv)
+                assert bool(got[sees][:, of].isnan().all())
+                near(got[~sees][:, of], want[~sees][:, of], tol[~sees][:, of])
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+def test_large_scores_and_constant_keys(ops, dtype):
+    """Scores far beyond what exp holds, keys all alike (step 0), a scale of 0."""
+    nh, nkv, hd, page, n = 8, 2, 64, 16, 70
+    gen = torch.Generator().manual_seed(4)
+    s = Sequences(ops, nh, nkv, hd, page, (n, n), gen, dtype)
+    x = torch.randn(n, 3 * nkv * hd, generator=gen)
+    x[:, nkv * hd:2 * nkv * hd] = 0.75
+    ops.rope_cache4(x.to(dtype).to(DEV), nkv, nkv, hd, s.cache, s.slots[1].to(torch.int32))
+    s.held = plain.parts(s.cache, nkv, hd)
+    q, out = queries(4, nh * hd, dtype, gen), torch.empty(4, nh * hd, dtype=dtype, device=DEV)
+    for scale in (hd ** -0.5, 200.0, 0.0):
+        ops.attention_decode4(q, out, s.cache, s.dev_tables, s.stride, ints([0, 1, 0, 1]), ints([n, n, 9, 9]), nh, nkv, hd, scale, n)
+        want, tol = s.expect(q, [0, 1, 0, 1], [(0, n), (0, n), (0, 9), (0, 9)], scale)
+        near(out, want, tol)
+
+
+def test_pages_that_are_none_hide_their_tokens(ops):
+    nh, nkv, hd, page = 4, 2, 64, 16
+    gen = torch.Generator().manual_seed(6)
+    s = Sequences(ops, nh, nkv, hd, page, (64, 64), gen, BF)
+    tables = s.dev_tables.clone().view(2, -1)
+    tables[0, 1], tables[1] = s.pages, -1
+    q, out = queries(2, nh * hd, BF, gen), torch.empty(2, nh * hd, dtype=BF, device=DEV)
+    ops.attention_decode4(q, out, s.cache, tables.view(-1), s.stride, ints([0, 1]), ints([64, 64]), nh, nkv, hd, 0.125, 64)
+    s.slots[0] = torch.cat([s.slots[0][:16], s.slots[0][32:]])
+    want, tol = s.expect(q, [0, -1], [(0, 48), (0, 0)], 0.125)
+    near(out, want, tol)
+    runs = torch.empty(2, nh * hd, dtype=BF, device=DEV)
+    ops.attention_prefill4(q, runs, s.cache, tables.view(-1), s.stride, ints([0, 1, 2]), ints([63, 63]), 2, 1, nh, nkv, hd, 0.125)
+    near(runs, want, tol)
