@@ -1,7 +1,26 @@
-// Attention over the 4-bit cache (cache4.h): softmax(scale * q . k) v over a row's visible tokens, max(0, p + 1 - window) <= t <= p.
+// Attention over the 4-bit cache (cache4.h): softmax(scale * q . k) v over a row's visible tokens, max(0, p + 1 - window) <= t <= p,
+// for rows of different sequences and for runs of consecutive positions.
 //
-// A wave takes one row of one head and walks its tokens 64 at a time with a running maximum m and sum l: a lane scores a token
-// of its own, q . (low + step c) = low * sum(q) + step * (q . c), and then adds up entries of its own over the 64 tokens.
+// The heads that share a kv head read the same keys: the rows of a walk are (position, head of the group) pairs, position by
+// position, 16 of them to a tile, RT tiles to a wave.  A single token of a sequence is a run of one.  A wave walks its tokens 32 at a
+// time with a running maximum m, on the matrix cores (16x16x32, bfloat16), both products transposed:
+//   S^T[token][row] = K[token][entry] Q^T[entry][row],   O^T[entry][row] += V^T[entry][token] P^T[token][row]
+// so that the scores of a lane all belong to one row (lane % 16) and are, as they stand, what the second product takes from that
+// lane.  Nothing passes through LDS.
+//
+// Codes become operands without arithmetic: 0x4300 | c is 128 + c in bfloat16, exactly, and one shift and one bit operation give two of them
+// (7 instructions for 8 codes; keys and values both lie in the order that this needs).  With k = low + step c,
+//   q . k = step (q . (128 + c) - 128 sum q) + low sum q         the sum of a row's q once, -128 times it as the accumulator's start
+//   sum p v = sum (p step) (128 + c) - 128 sum (p step) + sum p low
+// where p step is what is rounded to bfloat16 (float rows: split into three, which keep all 24 bits, as q is), and its sum comes from
+// one more matrix instruction with ones, so that the 128 cancel exactly as rounded; sum p and sum p low stay in 32 bits.
+//
+// How the work is laid out (a rule on sizes, `plan`):
+//   KEYS   the four waves of a workgroup share a tile of rows and take every fourth 32 tokens; their m, l, o meet in LDS.  For
+//          single tokens and short runs: their time is reading the cache.
+//   rows   the four waves have rows of their own and read the same keys at about the same time.  For runs of many rows.
+// and contexts are cut into segments that run as workgroups of their own while there are few; a second launch joins what they leave
+// in scratch (o, m, l in 32 bits, in the order of the segments).
 #include <cfloat>
 
 #include "cache4.h"
@@ -10,79 +29,536 @@
 namespace kvcm {
 namespace {
 
-template <class T, int HD, bool RUNS>
-__global__ void __launch_bounds__(kWave) attention4_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride,
-                                                           const uint8_t* __restrict__ cache, const int* __restrict__ tables, int table_stride, int seqs,
-                                                           const int* __restrict__ where, const int* __restrict__ lens, int nh, int nkv, int pages, int page,
-                                                           float scale, int window) {
-  __shared__ float qs[HD], ps[kWave];
-  __shared__ const uint8_t* tiles_at[kWave];
-  const int lane = threadIdx.x, head = blockIdx.y, kvh = head / (nh / nkv);
-  long long row;
-  int seq, ctx;
-  if constexpr (RUNS) {
-    seq = blockIdx.z;
-    row = where[seq] + static_cast<int>(blockIdx.x);
-    if (row >= where[seq + 1]) return;
-    ctx = lens[seq] + static_cast<int>(blockIdx.x) + 1;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kChunk = 32;      // tokens a wave takes at a time: two tiles of the cache
+
+__device__ __forceinline__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2)); }
+__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// 128 + c of the codes 4s .. 4s + 3 bits into either half of a word.
+__device__ __forceinline__ uint32_t codes(uint32_t word, int s) { return (word >> (4 * s) & 0x000F000Fu) | 0x43004300u; }
+
+// Numbers as sums of bfloat16 ones: one for rows of bfloat16, three for float (24 bits).
+template <class T> constexpr int kTerms = 1;
+template <> constexpr int kTerms<float> = 3;
+
+template <int N> struct Words { uint32_t w[N]; };
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    w[0] = x[0], w[1] = x[1];
   } else {
-    row = blockIdx.x;
-    seq = where[row];
-    ctx = static_cast<unsigned>(seq) < static_cast<unsigned>(seqs) ? lens[row] : 0;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p + 4 * i);
+      w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
+    }
   }
-  ctx = min(ctx, table_stride * page);
-  float sum_q = 0.f;
-  for (int d = lane; d < HD; d += kWave) {
-    qs[d] = load_f(q + row * q_stride + head * HD + d);
-    sum_q += qs[d];
+}
+
+// What a lane holds of 32 tokens: of either tile, a key's HD / 4 codes, four tokens' HD / 16 value codes, and the pairs of these four.
+template <int HD>
+struct Chunk {
+  uint32_t k[2][HD / 32], v[2][HD / 32];
+  u32x4 kp[2], vp[2];
+};
+
+// Where rows come from: single tokens (where = row_seq, lens = ctx_lens) or runs (run_start, seq_start).
+struct Rows {
+  const int *where, *lens;
+  int seqs, total;      // sequences with a table; rows
+  bool runs;
+};
+
+struct Shape {
+  int q_stride, out_stride, table_stride, nh, nkv, pages, page_tiles, page_shift;
+  float scale_log2;
+  int window, max_context, segment, tile_rows;
+  bool negate;      // a negative scale: of the queries
+};
+
+struct Span {
+  int row0, rows, seq, ctx0;      // first row, (position, head) pairs, sequence, context of the first row less one
+};
+
+// The run that unit (token or sequence) `unit` walks for; rows is 0 where there is none.
+__device__ __forceinline__ Span span_of(const Rows& r, const Shape& s, int unit) {
+  const int group = s.nh / s.nkv;
+  if (!r.runs) {
+    const int seq = r.where[unit];
+    return Span{unit, group, seq, static_cast<unsigned>(seq) < static_cast<unsigned>(r.seqs) ? max(0, r.lens[unit]) - 1 : -1};
   }
-  sum_q = wave_sum(sum_q);
-  float m = -FLT_MAX, l = 0.f, o[(HD + kWave - 1) / kWave] = {};
-  const int first = window > 0 ? max(0, ctx - window) : 0;
-  for (int t0 = first; t0 < ctx; t0 += kWave) {
-    const int t = t0 + lane;
-    float s = -FLT_MAX;
-    const uint8_t* tile = nullptr;
-    if (t < ctx) {
-      const unsigned pg = tables[static_cast<size_t>(seq) * table_stride + t / page];
-      if (pg < static_cast<unsigned>(pages)) {
-        tile = cache + ((static_cast<size_t>(pg) * nkv + kvh) * (page / kTile4) + t % page / kTile4) * tile4_bytes(HD);
-        const int i = t % kTile4;
-        float dot = 0.f;
-        for (int w = 0; w < HD / 8; ++w) {
-          const uint32_t c = reinterpret_cast<const uint32_t*>(tile + i * (HD / 2))[w];
-          for (int n = 0; n < 8; ++n) dot = fmaf(qs[8 * w + n], static_cast<float>(c >> (4 * n) & 15u), dot);
+  const int a = max(0, r.where[unit]), b = min(r.total, r.where[unit + 1]);
+  return Span{a, max(0, b - a) * group, unit, r.lens[unit]};
+}
+// Tokens that position i of a span sees: [first, end).
+__device__ __forceinline__ int end_of(const Span& p, const Shape& s, int i) { return max(0, min(p.ctx0 + i + 1, s.max_context)); }
+__device__ __forceinline__ int first_of(const Span& p, const Shape& s, int i) {
+  const int end = end_of(p, s, i);
+  return s.window > 0 ? max(0, min(end, p.ctx0 + i + 1 - s.window)) : 0;
+}
+
+template <class T>
+__device__ __forceinline__ void load_eight(const T* p, float x[8]) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint16_t raw __attribute__((ext_vector_type(8), aligned(2)));
+    const raw r = *reinterpret_cast<const raw*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = bf16_bits_to_float(r[i]);
+  } else {
+    typedef float raw __attribute__((ext_vector_type(4), aligned(4)));
+    const raw a = reinterpret_cast<const raw*>(p)[0], b = reinterpret_cast<const raw*>(p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[i + 4] = b[i];
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void store_some(T* p, const float (&x)[N]) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint16_t raw __attribute__((ext_vector_type(N), aligned(2)));
+    raw r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = float_to_bf16_bits(x[i]);
+    *reinterpret_cast<raw*>(p) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = x[i];
+  }
+}
+
+// blockIdx.x: kv head (fastest: with eight of them each of the chip's eight parts keeps to one), then segment, then tile of rows;
+// blockIdx.y: token or sequence.
+constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what the registers are bounded for
+  return hd == 256 ? 1 : wide ? (rt == 1 ? 2 : 1) : hd == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 2;
+}
+template <class T, int HD, int RT, bool KEYS>
+__global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
+                                                              const int* __restrict__ tables, Rows rows, Shape sh, int max_segs, float* __restrict__ scratch) {
+  constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>;
+  const int kvh = blockIdx.x % sh.nkv, rest = blockIdx.x / sh.nkv, part = rest % max_segs;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, n16 = lane % 16, kq = lane / 16;
+  const int group = sh.nh / sh.nkv;
+  const Span span = span_of(rows, sh, blockIdx.y);
+  const int block_first = rest / max_segs * sh.tile_rows;      // of the span's pairs
+  if (block_first >= span.rows) return;
+  const int block_last = min(block_first + sh.tile_rows, span.rows) - 1;
+  // the workgroup's tokens, and the segment of them that it takes
+  const int block_lo = first_of(span, sh, block_first / group), block_hi = end_of(span, sh, block_last / group);
+  const int seg_lo = block_lo / sh.segment, segs = block_hi > block_lo ? (block_hi - 1) / sh.segment - seg_lo + 1 : 1;
+  if (part >= segs) return;
+  const int first = block_first + (KEYS ? 0 : wave * 16 * RT);
+  const int last = min(first + 16 * RT, span.rows) - 1;
+  if (!KEYS && first > block_last) return;      // (no barriers where waves have rows of their own)
+  const int seg_first = (seg_lo + part) * sh.segment, seg_end = seg_first + sh.segment;
+  const int lo = max(first_of(span, sh, first / group), seg_first), hi = min(end_of(span, sh, last / group), seg_end);
+  const int all_lo = first_of(span, sh, last / group), all_hi = end_of(span, sh, first / group);      // what every row of the wave sees
+
+  int row[RT], head[RT], row_lo[RT], row_hi[RT];
+  float q_sum[RT];
+  u32x4 qf[RT][NT][KS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int f = min(first + 16 * rt + n16, span.rows - 1);      // pairs past the end repeat the last one; they are never stored
+    row[rt] = span.row0 + f / group;
+    head[rt] = kvh * group + f % group;
+    row_lo[rt] = max(first_of(span, sh, f / group), seg_first);
+    row_hi[rt] = min(end_of(span, sh, f / group), seg_end);
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      float x[8];
+      load_eight(q + static_cast<size_t>(row[rt]) * sh.q_stride + head[rt] * HD + kq * (HD / 4) + 8 * c, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = sh.negate ? -x[i] : x[i];
+        sum += x[i];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {      // codes come in the order 0 4 1 5 2 6 3 7
+          qf[rt][n][c][i] = pack(x[i], x[i + 4]);
+          if (n + 1 < NT) {
+            x[i] -= bf16_bits_to_float(qf[rt][n][c][i] & 0xFFFFu);
+            x[i + 4] -= bf16_bits_to_float(qf[rt][n][c][i] >> 16);
+          }
         }
-        const uint32_t pair = reinterpret_cast<const uint32_t*>(tile + 8 * HD)[i];
-        s = scale * fmaf(step4(pair), dot, low4(pair) * sum_q);
+    }
+    q_sum[rt] = rows_sum(sum);
+  }
+
+  float m[RT], l[RT], of_low[RT];
+  f32x4 o[RT][C], of_step[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -FLT_MAX;
+    l[rt] = of_low[rt] = 0.f;
+    of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < C; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  constexpr int STRIDE = KEYS ? kWaves : 1;
+  const int chunk_first = lo / kChunk + (KEYS ? wave : 0), chunk_end = (hi + kChunk - 1) / kChunk;      // every STRIDE-th of them
+  const int* table = tables + static_cast<size_t>(max(span.seq, 0)) * sh.table_stride;      // (looked at only where there are tokens)
+  const int k_at = n16 * (HD / 2) + kq * (HD / 8), v_at = value4_at(HD) + (kq * 16 + n16) * (HD / 8);
+  const int kp_at = 8 * HD + kq * 16, vp_at = value4_at(HD) + 8 * HD + kq * 16;
+
+  struct Ids { int page[2]; };      // -1: no tokens there
+  auto ids_of = [&](int chunk) {
+    Ids r;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tile = 2 * chunk + j, p = sh.page_shift >= 0 ? tile >> sh.page_shift : tile / sh.page_tiles;
+      r.page[j] = tile * kTile4 < hi ? table[p] : -1;
+      if (static_cast<unsigned>(r.page[j]) >= static_cast<unsigned>(sh.pages)) r.page[j] = -1;
+    }
+    return r;
+  };
+  auto request = [&](int chunk, const Ids& ids, Chunk<HD>& c) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tile = 2 * chunk + j, in_page = sh.page_shift >= 0 ? tile & (sh.page_tiles - 1) : tile % sh.page_tiles;
+      // a tile without tokens: the cache's first, which nobody looks at
+      const uint8_t* p = cache + (ids.page[j] < 0 ? 0 : ((static_cast<size_t>(ids.page[j]) * sh.nkv + kvh) * sh.page_tiles + in_page) * tile4_bytes(HD));
+      load_words(p + k_at, c.k[j]);
+      c.kp[j] = *reinterpret_cast<const u32x4*>(p + kp_at);
+      load_words(p + v_at, c.v[j]);
+      c.vp[j] = *reinterpret_cast<const u32x4*>(p + vp_at);
+    }
+  };
+
+  auto multiply = [&](int chunk, const Ids& ids, const Chunk<HD>& c) {
+    const int t0 = chunk * kChunk;
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float start = -128.f * q_sum[rt];
+        s[rt][j] = f32x4{start, start, start, start};
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 kf{codes(c.k[j][k], 0), codes(c.k[j][k], 1), codes(c.k[j][k], 2), codes(c.k[j][k], 3)};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[rt][j] = product(kf, qf[rt][n][k], s[rt][j]);
       }
     }
-    const float m_new = fmaxf(m, wave_max(s));
-    const float p = tile != nullptr ? expf(s - m_new) : 0.f, alpha = expf(m - m_new);
-    m = m_new;
-    l = l * alpha + wave_sum(p);
-    __syncthreads();
-    ps[lane] = p;
-    tiles_at[lane] = tile;
-    __syncthreads();
-    for (int j = 0; j < (HD + kWave - 1) / kWave; ++j) {
-      const int d = lane + j * kWave;
-      o[j] *= alpha;
-      if (d >= HD) continue;
-      for (int k = 0; k < kWave; ++k) {
-        if (tiles_at[k] == nullptr) continue;
-        const uint8_t* values = tiles_at[k] + value4_at(HD);
-        const int i = (t0 + k) % kTile4;
-        const uint32_t pair = reinterpret_cast<const uint32_t*>(values + 8 * HD)[i];
-        int at = value4_byte<HD>(i, d / 4);
-        if constexpr (HD == 32) at += d % 4 / 2 * 4;
-        else at += d % 4 / 2;
-        o[j] = fmaf(ps[k], fmaf(step4(pair), static_cast<float>(values[at] >> (4 * (d % 2)) & 15), low4(pair)), o[j]);
+    const bool whole = t0 >= all_lo && t0 >= lo && t0 + kChunk <= min(all_hi, hi) && ids.page[0] >= 0 && ids.page[1] >= 0;
+    u32x4 pf[RT][NT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float mx = -FLT_MAX, p[2][4], p_step[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[rt][j][i] = fmaf(step4(c.kp[j][i]), s[rt][j][i], low4(c.kp[j][i]) * q_sum[rt]);
+      uint32_t seen = 0xFF;      // a bit for each of the lane's tokens
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = t0 + 16 * j + 4 * kq + i;
+            const bool ok = t >= row_lo[rt] && t < row_hi[rt] && ids.page[j] >= 0;
+            seen |= static_cast<uint32_t>(ok) << (4 * j + i);
+            s[rt][j][i] = ok ? s[rt][j][i] : -FLT_MAX;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][j][i]);
+      const float m_new = fmaxf(m[rt], rows_max(mx)), shift = -m_new * sh.scale_log2;
+      const float alpha = __builtin_amdgcn_exp2f((m[rt] - m_new) * sh.scale_log2);
+      m[rt] = m_new;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][j][i], sh.scale_log2, shift));
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {      // the maximum moves in few chunks
+        l[rt] *= alpha;
+        of_low[rt] *= alpha;
+        of_step[rt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < C; ++d) o[rt][d] *= alpha;
+      }
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            l[rt] += p[j][i];
+            of_low[rt] = fmaf(p[j][i], low4(c.vp[j][i]), of_low[rt]);
+            p_step[j][i] = p[j][i] * step4(c.vp[j][i]);
+          }
+      } else {
+        // zero times what a place that is not seen holds (an Inf, a NaN) would not be zero
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool ok = seen >> (4 * j + i) & 1;
+            l[rt] += ok ? p[j][i] : 0.f;
+            of_low[rt] += ok ? p[j][i] * low4(c.vp[j][i]) : 0.f;
+            p_step[j][i] = ok ? p[j][i] * step4(c.vp[j][i]) : 0.f;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t two = pack(p_step[j][2 * i], p_step[j][2 * i + 1]);
+            pf[rt][n][2 * j + i] = two;
+            if (n + 1 < NT) {
+              p_step[j][2 * i] -= bf16_bits_to_float(two & 0xFFFFu);
+              p_step[j][2 * i + 1] -= bf16_bits_to_float(two >> 16);
+            }
+          }
+    }
+    const u32x4 ones{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) of_step[rt] = product(ones, pf[rt][n], of_step[rt]);
+#pragma unroll
+    for (int d = 0; d < C; ++d) {
+      u32x4 vf;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          if constexpr (C == 2) vf[2 * j + pair] = codes(c.v[j][0], d + 2 * pair);
+          else vf[2 * j + pair] = codes(c.v[j][pair * (C / 4) + d / 4], d % 4);
+        }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[rt][d] = product(vf, pf[rt][n], o[rt][d]);
+    }
+  };
+
+  if (chunk_first < chunk_end) {
+    // page ids two chunks ahead, tokens one: a chunk past the end asks for the cache's first tile (no load behind a branch)
+    Chunk<HD> a, b;
+    Ids ids_a = ids_of(chunk_first), ids_b = ids_of(chunk_first + STRIDE);
+    request(chunk_first, ids_a, a);
+    int chunk = chunk_first;
+    while (true) {
+      request(chunk + STRIDE, ids_b, b);
+      Ids next = ids_of(chunk + 2 * STRIDE);
+      multiply(chunk, ids_a, a);
+      chunk += STRIDE;
+      if (chunk >= chunk_end) break;
+      ids_a = next;
+      request(chunk + STRIDE, ids_a, a);
+      next = ids_of(chunk + 2 * STRIDE);
+      multiply(chunk, ids_b, b);
+      chunk += STRIDE;
+      if (chunk >= chunk_end) break;
+      ids_b = next;
+    }
+  }
+
+  // o / l of a wave's rows, or (o, m, l) where waves or segments still have to be joined
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] = rows_sum(l[rt]);
+    const float add = rows_sum(of_low[rt]) - 128.f * of_step[rt][0];
+#pragma unroll
+    for (int d = 0; d < C; ++d) o[rt][d] += add;
+  }
+  if constexpr (!KEYS) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (first + 16 * rt + n16 >= span.rows) continue;
+      const float by = segs > 1 ? 1.f : l[rt] == 0.f ? 0.f : 1.f / l[rt];
+      float* left = segs > 1 ? scratch + ((static_cast<size_t>(row[rt]) * sh.nh + head[rt]) * max_segs + part) * (HD + 2) : nullptr;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {      // lane kq has entries kq * HD / 4 on
+        float x[C];
+#pragma unroll
+        for (int d = 0; d < C; ++d) x[d] = o[rt][d][i] * by;
+        const int at = (4 * kq + i) * C;
+        if (segs > 1) {
+#pragma unroll
+          for (int d = 0; d < C; ++d) left[at + d] = x[d];
+        } else {
+          store_some(out + static_cast<size_t>(row[rt]) * sh.out_stride + head[rt] * HD + at, x);
+        }
+      }
+      if (segs > 1 && kq == 0) {
+        left[HD] = m[rt];
+        left[HD + 1] = l[rt];
+      }
+    }
+  } else {
+    __shared__ float os[kWaves][16][HD + 4], ms[kWaves][16], ls[kWaves][16];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (rt > 0) __syncthreads();
+      if (kq == 0) {
+        ms[wave][n16] = m[rt];
+        ls[wave][n16] = l[rt];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < C; ++d) os[wave][n16][(4 * kq + i) * C + d] = o[rt][d][i];
+      __syncthreads();
+      constexpr int LANES = kThreads / 16, PER = HD / LANES;      // lanes of a row, entries of a lane
+      const int r = threadIdx.x / LANES, at = threadIdx.x % LANES * PER, f = first + 16 * rt + r;
+      if (f >= span.rows) continue;
+      float top = ms[0][r], sum = 0.f, x[PER] = {};
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ms[w][r]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float by = __builtin_amdgcn_exp2f((ms[w][r] - top) * sh.scale_log2);
+        sum = fmaf(ls[w][r], by, sum);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] = fmaf(os[w][r][at + e], by, x[e]);
+      }
+      const size_t to = span.row0 + f / group;
+      const int h = kvh * group + f % group;
+      if (segs > 1) {
+        float* left = scratch + ((to * sh.nh + h) * max_segs + part) * (HD + 2);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) left[at + e] = x[e];
+        if (at == 0) {
+          left[HD] = top;
+          left[HD + 1] = sum;
+        }
+      } else {
+        const float by = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] *= by;
+        store_some(out + to * sh.out_stride + h * HD + at, x);
       }
     }
   }
-  for (int j = 0; j < (HD + kWave - 1) / kWave; ++j)
-    if (lane + j * kWave < HD) store_f(out + row * out_stride + head * HD + lane + j * kWave, l == 0.f ? 0.f : o[j] / l);
+}
+
+// Joins the segments of a row: one wave a (row, head).
+template <class T, int HD>
+__global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ scratch, T* __restrict__ out, Rows rows, Shape sh, int max_segs) {
+  const int head = blockIdx.x, group = sh.nh / sh.nkv, lane = threadIdx.x;
+  const Span span = span_of(rows, sh, blockIdx.z);
+  const int at = blockIdx.y;      // position in the span
+  if (at * group >= span.rows) return;
+  const int f = at * group + head % group, block_first = f / sh.tile_rows * sh.tile_rows, block_last = min(block_first + sh.tile_rows, span.rows) - 1;
+  const int block_lo = first_of(span, sh, block_first / group), block_hi = end_of(span, sh, block_last / group);
+  const int segs = block_hi > block_lo ? (block_hi - 1) / sh.segment - block_lo / sh.segment + 1 : 1;
+  if (segs == 1) return;
+  const size_t row = span.row0 + at;
+  const float* left = scratch + (row * sh.nh + head) * max_segs * (HD + 2);
+  float top = -FLT_MAX;
+  for (int i = 0; i < segs; ++i) top = fmaxf(top, left[i * (HD + 2) + HD]);
+  constexpr int PER = (HD + kWave - 1) / kWave;
+  float sum = 0.f, x[PER] = {};
+  for (int i = 0; i < segs; ++i, left += HD + 2) {
+    const float by = __builtin_amdgcn_exp2f((left[HD] - top) * sh.scale_log2);
+    sum = fmaf(left[HD + 1], by, sum);
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (lane + e * kWave < HD) x[e] = fmaf(left[lane + e * kWave], by, x[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e)
+    if (lane + e * kWave < HD) store_f(out + row * sh.out_stride + head * HD + lane + e * kWave, sum == 0.f ? 0.f : x[e] / sum);
+}
+
+// ---- host side
+struct Plan {
+  int rt, segment, max_segs, tile_rows, tiles;
+  bool keys;
+  long long floats;
+};
+
+constexpr long long kFill = 512;      // workgroups that fill the chip: two on each of 256 CUs
+
+Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
+  Plan p{};
+  const int group = nh / nkv;
+  const long long pairs = static_cast<long long>(max_run) * group;
+  const long long waves = static_cast<long long>(units) * nkv * ((pairs + 31) / 32);
+  p.keys = pairs <= 16 || waves < 2 * kFill;
+  p.rt = p.keys ? (pairs > 16 && hd <= 128 ? 2 : 1) : 2;
+  if (hd == 256) p.rt = 1;
+  p.tile_rows = 16 * p.rt * (p.keys ? 1 : kWaves);
+  p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
+  const long long groups = static_cast<long long>(units) * nkv * p.tiles;
+  const long long seen = window > 0 && window + p.tile_rows < max_context ? window + p.tile_rows : max_context;
+  long long parts = (kFill + groups - 1) / groups;
+  const int least = 8 * kChunk;      // tokens of a segment at least
+  if (parts > (seen + least - 1) / least) parts = (seen + least - 1) / least;
+  if (parts < 1) parts = 1;
+  p.segment = static_cast<int>(((seen + parts - 1) / parts + least - 1) / least * least);
+  if (p.segment < least) p.segment = least;
+  if (parts == 1) p.segment = 0x7FFFFFFF;
+  p.max_segs = parts == 1 ? 1 : static_cast<int>((max_context + p.segment - 1) / p.segment);
+  if (parts > 1 && seen < max_context) p.max_segs = static_cast<int>((seen - 1) / p.segment + 2);
+  p.floats = p.max_segs == 1 ? 0 : static_cast<long long>(T) * nh * p.max_segs * (hd + 2);
+  return p;
+}
+
+int launch(const char* what, const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride, Rows rows,
+           int units, int max_run, int nh, int nkv, int hd, int pages, int page, float scale, int window, int max_context, float* scratch, long long scratch_floats,
+           hipStream_t stream) {
+  KVCM_REQUIRE(kvcm_cache4_supported(nh, nkv, hd, page), "%s: heads %d, kv heads %d, head_dim %d, pages of %d tokens are not taken", what, nh, nkv, hd, page);
+  KVCM_REQUIRE(dtype == kF32 || dtype == kBF16, "%s: dtype %d", what, dtype);
+  KVCM_REQUIRE(pages > 0 && static_cast<long long>(pages) * page < (1ll << 31), "%s: %d pages of %d tokens", what, pages, page);
+  KVCM_REQUIRE(table_stride > 0 && rows.seqs > 0 && static_cast<long long>(table_stride) * page < (1ll << 31), "%s: %d tables of %d pages", what, rows.seqs, table_stride);
+  KVCM_REQUIRE(nh < 65536 && q_stride >= nh * hd && out_stride >= nh * hd && window >= 0 && max_context >= 0, "%s: rows of %d and %d entries, window %d, contexts up to %d",
+               what, q_stride, out_stride, window, max_context);
+  KVCM_REQUIRE(rows.total > 0 && max_run > 0, "%s: %d rows, runs of up to %d", what, rows.total, max_run);
+  KVCM_REQUIRE(q != nullptr && out != nullptr && cache != nullptr && tables != nullptr && rows.where != nullptr && rows.lens != nullptr, "%s: null operand", what);
+  const Plan p = plan(units, rows.total, max_run, nh, nkv, hd, max_context, window);
+  KVCM_REQUIRE(p.floats == 0 || (scratch != nullptr && scratch_floats >= p.floats), "%s: scratch of %lld floats is needed", what, p.floats);
+  const int page_tiles = page / kTile4;
+  Shape s{q_stride, out_stride, table_stride, nh, nkv, pages, page_tiles, -1, fabsf(scale) * 1.4426950408889634f, window,
+          static_cast<int>(static_cast<long long>(table_stride) * page < max_context ? table_stride * page : max_context), p.segment, p.tile_rows, scale < 0.f};
+  if ((page_tiles & (page_tiles - 1)) == 0) s.page_shift = __builtin_ctz(page_tiles);
+  if (s.scale_log2 == 0.f) s.scale_log2 = 1e-30f;      // (0 times what has not seen a token yet would not be 0)
+  const long long x = static_cast<long long>(nkv) * p.max_segs * p.tiles;
+  KVCM_REQUIRE(x < (1ll << 31) && units < 65536, "%s: %lld workgroups for each of %d sequences", what, x, units);
+  KVCM_REQUIRE(p.max_segs == 1 || max_run < 65536, "%s: runs of %d rows cut into segments", what, max_run);
+  const dim3 grid(static_cast<unsigned>(x), units);
+  KVCM_HEAD4(hd, {
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      const T* qt = static_cast<const T*>(q);
+      T* ot = static_cast<T*>(out);
+      const uint8_t* ct = static_cast<const uint8_t*>(cache);
+      if constexpr (HD < 256) {
+        if (p.rt == 2 && p.keys) attention4_kernel<T, HD, 2, true><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
+        if (p.rt == 2 && !p.keys) attention4_kernel<T, HD, 2, false><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
+      }
+      if (p.rt == 1 && p.keys) attention4_kernel<T, HD, 1, true><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
+      if (HD == 256 && p.rt == 1 && !p.keys) attention4_kernel<T, 256, 1, false><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
+      if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), kWave, 0, stream>>>(scratch, ot, rows, s, p.max_segs);
+    };
+    if (dtype == kBF16) go(bf16_t());
+    else go(float());
+  });
+  return launch_status(what);
 }
 
 }  // namespace
@@ -90,59 +566,32 @@ __global__ void __launch_bounds__(kWave) attention4_kernel(const T* __restrict__
 
 using namespace kvcm;
 
-namespace {
-
-int check(const char* what, const void* q, int dtype, int q_stride, const void* out, int out_stride, const void* cache, const int* tables, int table_stride, int seqs,
-          const int* a, const int* b, int nh, int nkv, int hd, int pages, int page, int window) {
-  KVCM_REQUIRE(kvcm_cache4_supported(nh, nkv, hd, page), "%s: heads %d, kv heads %d, head_dim %d, pages of %d tokens are not taken", what, nh, nkv, hd, page);
-  KVCM_REQUIRE(dtype == kF32 || dtype == kBF16, "%s: dtype %d", what, dtype);
-  KVCM_REQUIRE(pages > 0 && static_cast<long long>(pages) * page < (1ll << 31), "%s: %d pages of %d tokens", what, pages, page);
-  KVCM_REQUIRE(table_stride > 0 && seqs > 0 && static_cast<long long>(table_stride) * page < (1ll << 31), "%s: %d tables of %d pages", what, seqs, table_stride);
-  KVCM_REQUIRE(q_stride >= nh * hd && out_stride >= nh * hd && window >= 0 && nh < 65536 && seqs < 65536, "%s: rows of %d and %d entries, window %d", what, q_stride, out_stride, window);
-  KVCM_REQUIRE(q != nullptr && out != nullptr && cache != nullptr && tables != nullptr && a != nullptr && b != nullptr, "%s: null operand", what);
-  return 0;
-}
-
-}  // namespace
-
 extern "C" {
 
-long long kvcm_attention_decode4_scratch(int, int, int, int, int, int) { return 0; }
-
-int kvcm_attention_decode4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride, int seqs,
-                           const int* row_seq, const int* ctx_lens, int T, int nh, int nkv, int hd, int pages, int page, float scale, int window, int, float*,
-                           long long, hipStream_t stream) {
-  if (T == 0) return 0;
-  if (check("attention_decode4", q, dtype, q_stride, out, out_stride, cache, tables, table_stride, seqs, row_seq, ctx_lens, nh, nkv, hd, pages, page, window)) return -1;
-  KVCM_REQUIRE(T > 0, "attention_decode4: %d rows", T);
-  KVCM_HEAD4(hd, {
-    if (dtype == kBF16)
-      attention4_kernel<bf16_t, HD, false><<<dim3(T, nh), kWave, 0, stream>>>(static_cast<const bf16_t*>(q), q_stride, static_cast<bf16_t*>(out), out_stride,
-          static_cast<const uint8_t*>(cache), tables, table_stride, seqs, row_seq, ctx_lens, nh, nkv, pages, page, scale, window);
-    else
-      attention4_kernel<float, HD, false><<<dim3(T, nh), kWave, 0, stream>>>(static_cast<const float*>(q), q_stride, static_cast<float*>(out), out_stride,
-          static_cast<const uint8_t*>(cache), tables, table_stride, seqs, row_seq, ctx_lens, nh, nkv, pages, page, scale, window);
-  });
-  return launch_status("attention_decode4");
+long long kvcm_attention_decode4_scratch(int T, int nh, int nkv, int hd, int max_context, int window) {
+  if (T <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0) return 0;
+  return plan(T, T, 1, nh, nkv, hd, max_context, window).floats;
 }
 
-long long kvcm_attention_prefill4_scratch(int, int, int, int, int, int, int, int) { return 0; }
+int kvcm_attention_decode4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride, int seqs,
+                           const int* row_seq, const int* ctx_lens, int T, int nh, int nkv, int hd, int pages, int page, float scale, int window, int max_context,
+                           float* scratch, long long scratch_floats, hipStream_t stream) {
+  if (T == 0) return 0;
+  return launch("attention_decode4", q, dtype, q_stride, out, out_stride, cache, tables, table_stride, Rows{row_seq, ctx_lens, seqs, T, false}, T, 1, nh, nkv, hd, pages,
+                page, scale, window, max_context, scratch, scratch_floats, stream);
+}
+
+long long kvcm_attention_prefill4_scratch(int T, int nh, int nkv, int hd, int max_context, int max_run, int num_seqs, int window) {
+  if (T <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || max_run <= 0 || num_seqs <= 0) return 0;
+  return plan(num_seqs, T, max_run, nh, nkv, hd, max_context, window).floats;
+}
 
 int kvcm_attention_prefill4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride,
                             const int* run_start, const int* seq_start, int num_seqs, int max_run, int T, int nh, int nkv, int hd, int pages, int page, float scale,
-                            int window, int, float*, long long, hipStream_t stream) {
+                            int window, int max_context, float* scratch, long long scratch_floats, hipStream_t stream) {
   if (T == 0 || num_seqs == 0 || max_run == 0) return 0;
-  if (check("attention_prefill4", q, dtype, q_stride, out, out_stride, cache, tables, table_stride, num_seqs, run_start, seq_start, nh, nkv, hd, pages, page, window)) return -1;
-  KVCM_REQUIRE(T > 0 && max_run > 0, "attention_prefill4: %d rows, runs of up to %d", T, max_run);
-  KVCM_HEAD4(hd, {
-    if (dtype == kBF16)
-      attention4_kernel<bf16_t, HD, true><<<dim3(max_run, nh, num_seqs), kWave, 0, stream>>>(static_cast<const bf16_t*>(q), q_stride, static_cast<bf16_t*>(out),
-          out_stride, static_cast<const uint8_t*>(cache), tables, table_stride, num_seqs, run_start, seq_start, nh, nkv, pages, page, scale, window);
-    else
-      attention4_kernel<float, HD, true><<<dim3(max_run, nh, num_seqs), kWave, 0, stream>>>(static_cast<const float*>(q), q_stride, static_cast<float*>(out),
-          out_stride, static_cast<const uint8_t*>(cache), tables, table_stride, num_seqs, run_start, seq_start, nh, nkv, pages, page, scale, window);
-  });
-  return launch_status("attention_prefill4");
+  return launch("attention_prefill4", q, dtype, q_stride, out, out_stride, cache, tables, table_stride, Rows{run_start, seq_start, num_seqs, T, true}, num_seqs, max_run,
+                nh, nkv, hd, pages, page, scale, window, max_context, scratch, scratch_floats, stream);
 }
 
 }  // extern "C"
