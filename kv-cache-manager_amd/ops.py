@@ -312,7 +312,7 @@ _SYNC_LAUNCHES = bool(int(os.environ.get("KVCM_SYNC_LAUNCHES", "0") or 0))
 
 def _call(name, *args):
     """Calls a launching entry; while a program records, notes the call there first."""
-    fn = getattr(lib(), name)
+    fn = getattr(_lib or lib(), name)
     if _recording is not None:
         _recording.add(name, _slots(fn, args))
     if _SYNC_LAUNCHES:
@@ -342,9 +342,10 @@ def _dev(*ts):
 def _i32(t, name, n=None):
     if t is None:
         return
-    _need(t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 tensor")
-    if n is not None:
-        _need(t.numel() >= n, f"{name} holds {t.numel()} entries, {n} are needed")
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if n is not None and t.numel() < n:
+        raise ValueError(f"{name} holds {t.numel()} entries, {n} are needed")
 
 
 def _rows2d(t, name):
@@ -1217,39 +1218,52 @@ def cache4_supported(nh, nkv, hd, dtype, block_size=16):
     return dtype in _DT and bool(lib().kvcm_cache4_supported(nh, nkv, hd, block_size))
 
 
+_HEADS4 = (32, 64, 128, 256)
+
+
 def cache4_shape(pages, nkv, hd, block_size=16):
     """The shape of a 4-bit cache, a uint8 tensor: tiles of 16 tokens of one kv head, ``hd`` + 8 bytes a token for its key and its value.
     Each of the two is kept as 4-bit codes between its own smallest and largest entry: value = low + step * code, with low and step in
     bfloat16 and step a fifteenth of the range, so that an entry is off by about half a step at most.  A vector that holds an Inf or a
     NaN reads as NaN."""
-    _need(pages > 0 and nkv > 0 and hd in (32, 64, 128, 256) and block_size > 0 and block_size % 16 == 0,
+    _need(pages > 0 and nkv > 0 and hd in _HEADS4 and block_size > 0 and block_size % 16 == 0,
           "a 4-bit cache has pages of a multiple of 16 tokens and head_dim 32, 64, 128 or 256")
     return (pages, nkv, block_size // 16, 16 * (hd + 8))
 
 
 def _one_gpu(*ts):
     """Launches go to device 0's current stream: every operand lives there, and it is the current device."""
-    _dev(*ts)
     for t in ts:
-        _need(t is None or t.get_device() == 0, "kernel operands must live on device 0")
-    _need(torch.cuda.current_device() == 0, "device 0 must be the current device")
+        if t is not None and t.get_device() != 0:
+            _dev(t)
+            raise ValueError("kernel operands must live on device 0")
+    if torch._C._cuda_getDevice() != 0:
+        raise ValueError("device 0 must be the current device")
 
 
+# (These checks run before every launch; a message is made only when it is needed: one made on every call costs as much as the check.)
 def _check_cache4(cache, nkv, hd, nh=None):
-    _need(cache.dtype == torch.uint8 and cache.dim() == 4 and cache.is_contiguous() and cache.data_ptr() % 16 == 0
-          and tuple(cache.shape) == cache4_shape(cache.shape[0], nkv, hd, 16 * cache.shape[2]),
-          "the cache must be contiguous uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)], aligned to 16 bytes (cache4_shape)")
-    _need(cache.shape[0] * cache.shape[2] * 16 < 2 ** 31, "a cache of 2^31 token slots or more does not fit 32-bit slot numbers")
-    _need(nh is None or (nh > 0 and nh % nkv == 0), "the heads must be a multiple of the kv heads")
-    return cache.shape[0], 16 * cache.shape[2]
+    s = cache.shape
+    if not (cache.dtype == torch.uint8 and len(s) == 4 and s[1] == nkv > 0 and hd in _HEADS4 and s[3] == 16 * (hd + 8) and s[0] > 0 and s[2] > 0
+            and cache.is_contiguous() and cache.data_ptr() % 16 == 0):
+        raise ValueError("the cache must be contiguous uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)], aligned to 16 bytes (cache4_shape)")
+    if s[0] * s[2] >= 2 ** 27:
+        raise ValueError("a cache of 2^31 token slots or more does not fit 32-bit slot numbers")
+    if nh is not None and (nh <= 0 or nh % nkv):
+        raise ValueError("the heads must be a multiple of the kv heads")
+    return s[0], 16 * s[2]
 
 
 def _long_rows(t, name, rows, cols, dtype=None):
-    _rows2d(t, name)
-    _need(t.dtype in _DT and (dtype is None or t.dtype == dtype), f"{name} must be {'bfloat16 or float32' if dtype is None else dtype}")
-    _need(t.shape[0] >= rows >= 0 and t.shape[1] >= cols and (t.stride(0) >= cols or rows <= 1) and t.stride(0) < 2 ** 31,
-          f"{name} must be [>= {rows}, >= {cols}] with rows of their own")
-    return max(t.stride(0), cols)      # (a single row's stride may be anything)
+    """The stride of a matrix of rows (a single row's may be anything)."""
+    s, st = t.shape, t.stride()
+    if len(s) != 2 or (st[1] != 1 and s[1] > 1):
+        raise ValueError(f"{name} must be 2-d with unit inner stride")
+    if t.dtype not in _DT or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be {'bfloat16 or float32' if dtype is None else dtype}")
+    if not (s[0] >= rows >= 0 and s[1] >= cols and (st[0] >= cols or rows <= 1) and st[0] < 2 ** 31):
+        raise ValueError(f"{name} must be [>= {rows}, >= {cols}] with rows of their own")
+    return max(st[0], cols)
 
 
 def rope_cache4(qkv, nh, nkv, hd, cache, slots, cos_sin=None, q_out=None, rows=None):
@@ -1287,11 +1301,16 @@ def cache4_rows(cache, slots, k, v, rows=None):
 
 
 def _scratch4(what, need, scratch, device):
-    if need and scratch is None:
-        _need(_recording is None, f"{what}: a recorded step must bring its scratch (an allocation here would not outlive the step)")
-        scratch = torch.empty(need, dtype=torch.float32, device=device)
-    _need(scratch is None or (scratch.dtype == torch.float32 and scratch.is_contiguous()), "scratch must be contiguous float32")
-    _need(scratch is None or scratch.numel() >= need, f"{what}: scratch of {need} floats is needed")
+    if scratch is None:
+        if not need:
+            return None
+        if _recording is not None:
+            raise ValueError(f"{what}: a recorded step must bring its scratch (an allocation here would not outlive the step)")
+        return torch.empty(need, dtype=torch.float32, device=device)
+    if scratch.dtype != torch.float32 or not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous float32")
+    if scratch.numel() < need:
+        raise ValueError(f"{what}: scratch of {need} floats is needed")
     return scratch
 
 
