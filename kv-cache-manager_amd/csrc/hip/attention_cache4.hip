@@ -8,20 +8,29 @@
 // so that the scores of a lane all belong to one row (lane % 16) and are, as they stand, what the second product takes from that
 // lane.  Nothing passes through LDS.
 //
-// Codes become operands without arithmetic: 0x4300 | c is 128 + c in bfloat16, exactly, and one shift and one bit operation give two of them
-// (7 instructions for 8 codes; keys and values both lie in the order that this needs).  With k = low + step c,
-//   q . k = step (q . (128 + c) - 128 sum q) + low sum q         the sum of a row's q once, -128 times it as the accumulator's start
-//   sum p v = sum (p step) (128 + c) - 128 sum (p step) + sum p low
+// Codes become operands without arithmetic: in bfloat16 0x4300 | c is 128 + c and 0x4180 | c << 3 is 16 + c, exactly, and one shift and one
+// bit operation give two of them (7 or 8 instructions for 8 codes; keys and values both lie in the order that this needs).  Rows of
+// bfloat16 take B = 128, float rows, whose 32 bits the larger numbers would eat into, B = 16.  With k = mid + step (c - 8), where mid =
+// low + 8 step is the middle of a vector's range,
+//   q . k = step (q . (B + c) - (B + 8) sum q) + mid sum q         the sum of a row's q once, -(B + 8) times it as the accumulator's start
+//   sum p v = sum (p step) (B + c) - (B + 8) sum (p step) + sum p mid
 // where p step is what is rounded to bfloat16 (float rows: split into three, which keep all 24 bits, as q is), and its sum comes from
-// one more matrix instruction with ones, so that the 128 cancel exactly as rounded; sum p and sum p low stay in 32 bits.
+// one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0
+// as the values are from their middle.  sum p and sum p mid stay in 32 bits.
 //
 // How the work is laid out (a rule on sizes, `plan`):
-//   KEYS   the four waves of a workgroup share a tile of rows and take every fourth 32 tokens; their m, l, o meet in LDS.  For
-//          single tokens and short runs: their time is reading the cache.
-//   rows   the four waves have rows of their own and read the same keys at about the same time.  For runs of many rows.
+//   KEYS   the waves of a workgroup share a tile of rows and take every W-th 32 tokens; their m, l, o meet in LDS.  For single
+//          tokens and short runs: their time is reading the cache.
+//   rows   a wave has rows of its own.  For runs of many rows: vector instructions bound it (some 120 of a wave for 16 rows and 32
+//          tokens of 64 entries beside 9 matrix instructions).
 // and contexts are cut into segments that run as workgroups of their own while there are few; a second launch joins what they leave
 // in scratch (o, m, l in 32 bits, in the order of the segments).
+//
+// The maximum m that a row's exponentials are taken against is not the largest score but one that no score passes by more than 2^6: it
+// moves in few chunks, and only then do a row's four lanes compare what they have and the sums get scaled.
+#include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "cache4.h"
 #include "kvcm_hip.h"
@@ -36,19 +45,27 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kChunk = 32;      // tokens a wave takes at a time: two tiles of the cache
+constexpr float kAhead = 6.f;   // the maximum that a row's exponentials are taken against follows when a score is 2^6 ahead of it
 
 __device__ __forceinline__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2)); }
 __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// 128 + c of the codes 4s .. 4s + 3 bits into either half of a word.
-__device__ __forceinline__ uint32_t codes(uint32_t word, int s) { return (word >> (4 * s) & 0x000F000Fu) | 0x43004300u; }
+// B + c of the codes 4s .. 4s + 3 bits into either half of a word: one bit operation takes the mask and B, where one of them lies in a vector
+// register (`mask`; an instruction reads one scalar register).
+template <int B> constexpr uint32_t kMask = B == 128 ? 0x000F000Fu : 0x00780078u;
+template <int B>
+__device__ __forceinline__ uint32_t codes(uint32_t word, int s, uint32_t mask) {
+  if constexpr (B == 128) return (word >> (4 * s) & mask) | 0x43004300u;
+  return ((s == 0 ? word << 3 : word >> (4 * s - 3)) & mask) | 0x41804180u;
+}
 
 // Numbers as sums of bfloat16 ones: one for rows of bfloat16, three for float (24 bits).
 template <class T> constexpr int kTerms = 1;
 template <> constexpr int kTerms<float> = 3;
+template <class T> constexpr int kBias = 128;
+template <> constexpr int kBias<float> = 16;
 
 template <int N> struct Words { uint32_t w[N]; };
 template <int N>
@@ -81,10 +98,24 @@ struct Rows {
   bool runs;
 };
 
+// Division by a number that the host knows: a single token's walk is a few microseconds long, and dividing by a variable takes some
+// twenty instructions each time.  n / d = 2 n * by / 2^32 / 2^shift with by = 2^(31 + shift) / d rounded up, shift = log2 d rounded down:
+// too much by less than n / 2^(31 + shift) * d / d, below 1 / d for n < 2^30.
+struct Divisor {
+  int d, shift;
+  unsigned by;
+};
+inline Divisor divisor(int d) {
+  const int shift = 31 - __builtin_clz(d);
+  return Divisor{d, shift, static_cast<unsigned>(((1ull << (31 + shift)) + d - 1) / d)};
+}
+__device__ __forceinline__ int quotient(int n, const Divisor& d) { return static_cast<int>(__umulhi(2u * n, d.by) >> d.shift); }
+
 struct Shape {
-  int q_stride, out_stride, table_stride, nh, nkv, pages, page_tiles, page_shift;
+  int q_stride, out_stride, table_stride, nh, pages, max_segs, tiles;
+  Divisor nkv, group, segs, page_tiles, segment;      // segment: in chunks (and max_segs 1: not looked at)
   float scale_log2;
-  int window, max_context, segment, tile_rows;
+  int window, max_context, tile_rows;
   bool negate;      // a negative scale: of the queries
 };
 
@@ -94,19 +125,29 @@ struct Span {
 
 // The run that unit (token or sequence) `unit` walks for; rows is 0 where there is none.
 __device__ __forceinline__ Span span_of(const Rows& r, const Shape& s, int unit) {
-  const int group = s.nh / s.nkv;
   if (!r.runs) {
     const int seq = r.where[unit];
-    return Span{unit, group, seq, static_cast<unsigned>(seq) < static_cast<unsigned>(r.seqs) ? max(0, r.lens[unit]) - 1 : -1};
+    return Span{unit, s.group.d, seq, static_cast<unsigned>(seq) < static_cast<unsigned>(r.seqs) ? max(0, r.lens[unit]) - 1 : -1};
   }
   const int a = max(0, r.where[unit]), b = min(r.total, r.where[unit + 1]);
-  return Span{a, max(0, b - a) * group, unit, r.lens[unit]};
+  return Span{a, max(0, b - a) * s.group.d, unit, min(r.lens[unit], 0x7FFFFFFF - r.total)};
 }
 // Tokens that position i of a span sees: [first, end).
 __device__ __forceinline__ int end_of(const Span& p, const Shape& s, int i) { return max(0, min(p.ctx0 + i + 1, s.max_context)); }
 __device__ __forceinline__ int first_of(const Span& p, const Shape& s, int i) {
   const int end = end_of(p, s, i);
   return s.window > 0 ? max(0, min(end, p.ctx0 + i + 1 - s.window)) : 0;
+}
+
+// Which segments the tokens of a tile of rows lie in.
+struct Cut {
+  int first, segs;
+};
+__device__ __forceinline__ Cut cut_of(const Span& p, const Shape& s, int block_first, int block_last) {
+  if (s.max_segs == 1) return Cut{0, 1};
+  const int lo = first_of(p, s, quotient(block_first, s.group)), hi = end_of(p, s, quotient(block_last, s.group));
+  const int first = quotient(lo / kChunk, s.segment);
+  return Cut{first, hi > lo ? quotient((hi - 1) / kChunk, s.segment) - first + 1 : 1};
 }
 
 template <class T>
@@ -137,43 +178,47 @@ __device__ __forceinline__ void store_some(T* p, const float (&x)[N]) {
   }
 }
 
-// blockIdx.x: kv head (fastest: with eight of them each of the chip's eight parts keeps to one), then segment, then tile of rows;
-// blockIdx.y: token or sequence.
+// blockIdx.x: kv head (fastest: with eight of them each of the chip's eight parts keeps to one), then segment, then tile of rows, the last
+// tile first (it sees the most keys); blockIdx.y: token or sequence.
 constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what the registers are bounded for
   return hd == 256 ? 1 : wide ? (rt == 1 ? 2 : 1) : hd == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 2;
 }
-template <class T, int HD, int RT, bool KEYS>
-__global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
-                                                              const int* __restrict__ tables, Rows rows, Shape sh, int max_segs, float* __restrict__ scratch) {
-  constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>;
-  const int kvh = blockIdx.x % sh.nkv, rest = blockIdx.x / sh.nkv, part = rest % max_segs;
+template <class T, int HD, int RT, int W, bool KEYS>
+__global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
+                                                              const int* __restrict__ tables, Rows rows, Shape sh, float* __restrict__ scratch) {
+  constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>, B = kBias<T>;
+  const int rest = quotient(blockIdx.x, sh.nkv), kvh = blockIdx.x - rest * sh.nkv.d, tile_up = quotient(rest, sh.segs), part = rest - tile_up * sh.max_segs;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, n16 = lane % 16, kq = lane / 16;
-  const int group = sh.nh / sh.nkv;
+  const int group = sh.group.d;
   const Span span = span_of(rows, sh, blockIdx.y);
-  const int block_first = rest / max_segs * sh.tile_rows;      // of the span's pairs
+  const int block_first = (sh.tiles - 1 - tile_up) * sh.tile_rows;      // of the span's pairs
   if (block_first >= span.rows) return;
   const int block_last = min(block_first + sh.tile_rows, span.rows) - 1;
   // the workgroup's tokens, and the segment of them that it takes
-  const int block_lo = first_of(span, sh, block_first / group), block_hi = end_of(span, sh, block_last / group);
-  const int seg_lo = block_lo / sh.segment, segs = block_hi > block_lo ? (block_hi - 1) / sh.segment - seg_lo + 1 : 1;
+  const Cut cut = cut_of(span, sh, block_first, block_last);
+  const int segs = cut.segs;
   if (part >= segs) return;
   const int first = block_first + (KEYS ? 0 : wave * 16 * RT);
   const int last = min(first + 16 * RT, span.rows) - 1;
   if (!KEYS && first > block_last) return;      // (no barriers where waves have rows of their own)
-  const int seg_first = (seg_lo + part) * sh.segment, seg_end = seg_first + sh.segment;
-  const int lo = max(first_of(span, sh, first / group), seg_first), hi = min(end_of(span, sh, last / group), seg_end);
-  const int all_lo = first_of(span, sh, last / group), all_hi = end_of(span, sh, first / group);      // what every row of the wave sees
+  const int seg_first = sh.max_segs == 1 ? 0 : (cut.first + part) * sh.segment.d * kChunk;
+  const int seg_end = sh.max_segs == 1 ? 0x7FFFFFFF : static_cast<int>(min(0x7FFFFFFFu, static_cast<unsigned>(seg_first) + sh.segment.d * kChunk));
+  const int at_first = quotient(first, sh.group), at_last = quotient(last, sh.group);
+  const int lo = max(first_of(span, sh, at_first), seg_first), hi = min(end_of(span, sh, at_last), seg_end);
+  const int all_lo = first_of(span, sh, at_last), all_hi = end_of(span, sh, at_first);      // what every row of the wave sees
 
   int row[RT], head[RT], row_lo[RT], row_hi[RT];
   float q_sum[RT];
+  f32x4 start[RT];
   u32x4 qf[RT][NT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int f = min(first + 16 * rt + n16, span.rows - 1);      // pairs past the end repeat the last one; they are never stored
-    row[rt] = span.row0 + f / group;
-    head[rt] = kvh * group + f % group;
-    row_lo[rt] = max(first_of(span, sh, f / group), seg_first);
-    row_hi[rt] = min(end_of(span, sh, f / group), seg_end);
+    const int at = quotient(f, sh.group);
+    row[rt] = span.row0 + at;
+    head[rt] = kvh * group + f - at * group;
+    row_lo[rt] = max(first_of(span, sh, at), seg_first);
+    row_hi[rt] = min(end_of(span, sh, at), seg_end);
     float sum = 0.f;
 #pragma unroll
     for (int c = 0; c < KS; ++c) {
@@ -196,129 +241,148 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
         }
     }
     q_sum[rt] = rows_sum(sum);
+    const float less = -(B + 8.f) * q_sum[rt];
+    start[rt] = f32x4{less, less, less, less};
   }
 
-  float m[RT], l[RT], of_low[RT];
+  float m[RT], l[RT], of_mid[RT];
   f32x4 o[RT][C], of_step[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -FLT_MAX;
-    l[rt] = of_low[rt] = 0.f;
+    l[rt] = of_mid[rt] = 0.f;
     of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < C; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  constexpr int STRIDE = KEYS ? kWaves : 1;
+  constexpr int STRIDE = KEYS ? W : 1;
   const int chunk_first = lo / kChunk + (KEYS ? wave : 0), chunk_end = (hi + kChunk - 1) / kChunk;      // every STRIDE-th of them
   const int* table = tables + static_cast<size_t>(max(span.seq, 0)) * sh.table_stride;      // (looked at only where there are tokens)
   const int k_at = n16 * (HD / 2) + kq * (HD / 8), v_at = value4_at(HD) + (kq * 16 + n16) * (HD / 8);
   const int kp_at = 8 * HD + kq * 16, vp_at = value4_at(HD) + 8 * HD + kq * 16;
+  uint32_t mask;
+  asm("v_mov_b32 %0, %1" : "=v"(mask) : "n"(kMask<B>));
 
-  struct Ids { int page[2]; };      // -1: no tokens there
+  // Of either tile of a chunk: where it lies, and whether it has tokens.  One past the end stands for the last, one whose page is none for
+  // the cache's first page (nobody looks at their tokens): no load and no address is behind a branch.
+  struct Ids {
+    size_t at[2];
+    bool some[2];
+  };
+  const int tile_end = (hi + kTile4 - 1) / kTile4;
   auto ids_of = [&](int chunk) {
     Ids r;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int tile = 2 * chunk + j, p = sh.page_shift >= 0 ? tile >> sh.page_shift : tile / sh.page_tiles;
-      r.page[j] = tile * kTile4 < hi ? table[p] : -1;
-      if (static_cast<unsigned>(r.page[j]) >= static_cast<unsigned>(sh.pages)) r.page[j] = -1;
+      const int tile = min(2 * chunk + j, tile_end - 1), p = quotient(tile, sh.page_tiles), page = table[p];
+      r.some[j] = 2 * chunk + j < tile_end && static_cast<unsigned>(page) < static_cast<unsigned>(sh.pages);
+      const unsigned of_cache = static_cast<unsigned>(page) < static_cast<unsigned>(sh.pages) ? page : 0;
+      r.at[j] = ((static_cast<size_t>(of_cache) * sh.nkv.d + kvh) * sh.page_tiles.d + (tile - p * sh.page_tiles.d)) * tile4_bytes(HD);
     }
     return r;
   };
-  auto request = [&](int chunk, const Ids& ids, Chunk<HD>& c) {
+  auto request_keys = [&](const Ids& ids, Chunk<HD>& c) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int tile = 2 * chunk + j, in_page = sh.page_shift >= 0 ? tile & (sh.page_tiles - 1) : tile % sh.page_tiles;
-      // a tile without tokens: the cache's first, which nobody looks at
-      const uint8_t* p = cache + (ids.page[j] < 0 ? 0 : ((static_cast<size_t>(ids.page[j]) * sh.nkv + kvh) * sh.page_tiles + in_page) * tile4_bytes(HD));
+      const uint8_t* p = cache + ids.at[j];
       load_words(p + k_at, c.k[j]);
       c.kp[j] = *reinterpret_cast<const u32x4*>(p + kp_at);
+    }
+  };
+  auto request_values = [&](const Ids& ids, Chunk<HD>& c) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint8_t* p = cache + ids.at[j];
       load_words(p + v_at, c.v[j]);
       c.vp[j] = *reinterpret_cast<const u32x4*>(p + vp_at);
     }
   };
 
-  auto multiply = [&](int chunk, const Ids& ids, const Chunk<HD>& c) {
-    const int t0 = chunk * kChunk;
-    f32x4 s[RT][2];
+  auto score = [&](const Chunk<HD>& c, f32x4 (&s)[RT][2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+      u32x4 kf[KS];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float start = -128.f * q_sum[rt];
-        s[rt][j] = f32x4{start, start, start, start};
-      }
+      for (int k = 0; k < KS; ++k) kf[k] = u32x4{codes<B>(c.k[j][k], 0, mask), codes<B>(c.k[j][k], 1, mask), codes<B>(c.k[j][k], 2, mask), codes<B>(c.k[j][k], 3, mask)};
+      if constexpr (NT == 1) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const u32x4 kf{codes(c.k[j][k], 0), codes(c.k[j][k], 1), codes(c.k[j][k], 2), codes(c.k[j][k], 3)};
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+          for (int rt = 0; rt < RT; ++rt) s[rt][j] = product(kf[k], qf[rt][0][k], k == 0 ? start[rt] : s[rt][j]);
+      } else {
+        // 32 bits are to be kept: the small terms first, by themselves
 #pragma unroll
-          for (int n = 0; n < NT; ++n) s[rt][j] = product(kf, qf[rt][n][k], s[rt][j]);
+        for (int rt = 0; rt < RT; ++rt) {
+          s[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int n = NT - 1; n > 0; --n)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) s[rt][j] = product(kf[k], qf[rt][n][k], s[rt][j]);
+          s[rt][j] += start[rt];
+#pragma unroll
+          for (int k = 0; k < KS; ++k) s[rt][j] = product(kf[k], qf[rt][0][k], s[rt][j]);
+        }
       }
     }
-    const bool whole = t0 >= all_lo && t0 >= lo && t0 + kChunk <= min(all_hi, hi) && ids.page[0] >= 0 && ids.page[1] >= 0;
-    u32x4 pf[RT][NT];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float step = step4(c.kp[j][i]), mid = fmaf(8.f, step, low4(c.kp[j][i]));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][j][i] = fmaf(step, s[rt][j][i], mid * q_sum[rt]);
+      }
+  };
+  // WHOLE: every row sees all 32 tokens
+  auto add = [&](auto whole, int chunk, const Ids& ids, const Chunk<HD>& c, f32x4 (&s)[RT][2]) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    bool ok[RT][2][4];
+    float mx[RT];
+    bool move = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float mx = -FLT_MAX, p[2][4], p_step[2][4];
+      mx[rt] = -FLT_MAX;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[rt][j][i] = fmaf(step4(c.kp[j][i]), s[rt][j][i], low4(c.kp[j][i]) * q_sum[rt]);
-      uint32_t seen = 0xFF;      // a bit for each of the lane's tokens
-      if (!whole) {
-        seen = 0;
+        for (int i = 0; i < 4; ++i) {
+          const int t = chunk * kChunk + 16 * j + 4 * kq + i;
+          ok[rt][j][i] = WHOLE || ((t >= row_lo[rt]) & (t < row_hi[rt]) & (ids.some[j]));
+          s[rt][j][i] = ok[rt][j][i] ? s[rt][j][i] : -FLT_MAX;
+          mx[rt] = fmaxf(mx[rt], s[rt][j][i]);
+        }
+      move |= (mx[rt] - m[rt]) * sh.scale_log2 > kAhead;
+    }
+    if (__builtin_amdgcn_ballot_w64(move)) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int t = t0 + 16 * j + 4 * kq + i;
-            const bool ok = t >= row_lo[rt] && t < row_hi[rt] && ids.page[j] >= 0;
-            seen |= static_cast<uint32_t>(ok) << (4 * j + i);
-            s[rt][j][i] = ok ? s[rt][j][i] : -FLT_MAX;
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][j][i]);
-      const float m_new = fmaxf(m[rt], rows_max(mx)), shift = -m_new * sh.scale_log2;
-      const float alpha = __builtin_amdgcn_exp2f((m[rt] - m_new) * sh.scale_log2);
-      m[rt] = m_new;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][j][i], sh.scale_log2, shift));
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {      // the maximum moves in few chunks
+      for (int rt = 0; rt < RT; ++rt) {
+        const float top = fmaxf(m[rt], rows_max(mx[rt])), alpha = __builtin_amdgcn_exp2f((m[rt] - top) * sh.scale_log2);
+        m[rt] = top;
         l[rt] *= alpha;
-        of_low[rt] *= alpha;
+        of_mid[rt] *= alpha;
         of_step[rt] *= alpha;
 #pragma unroll
         for (int d = 0; d < C; ++d) o[rt][d] *= alpha;
       }
-      if (whole) {
+    }
+    u32x4 pf[RT][NT];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+    for (int rt = 0; rt < RT; ++rt) {
+      const float shift = -m[rt] * sh.scale_log2;
+      float p_step[2][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            l[rt] += p[j][i];
-            of_low[rt] = fmaf(p[j][i], low4(c.vp[j][i]), of_low[rt]);
-            p_step[j][i] = p[j][i] * step4(c.vp[j][i]);
-          }
-      } else {
-        // zero times what a place that is not seen holds (an Inf, a NaN) would not be zero
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool ok = seen >> (4 * j + i) & 1;
-            l[rt] += ok ? p[j][i] : 0.f;
-            of_low[rt] += ok ? p[j][i] * low4(c.vp[j][i]) : 0.f;
-            p_step[j][i] = ok ? p[j][i] * step4(c.vp[j][i]) : 0.f;
-          }
-      }
+        for (int i = 0; i < 4; ++i) {
+          // zero times what a place that is not seen holds (an Inf, a NaN) would not be zero
+          const uint32_t pair = ok[rt][j][i] ? c.vp[j][i] : 0u;
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[rt][j][i], sh.scale_log2, shift)), p = ok[rt][j][i] ? e : 0.f;
+          l[rt] += p;
+          const float step = step4(pair);
+          of_mid[rt] = fmaf(p, fmaf(8.f, step, low4(pair)), of_mid[rt]);
+          p_step[j][i] = p * step;
+        }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -335,9 +399,11 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
     }
     const u32x4 ones{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) {
+      if constexpr (NT > 1) of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < NT; ++n) of_step[rt] = product(ones, pf[rt][n], of_step[rt]);
+      for (int n = NT - 1; n >= 0; --n) of_step[rt] = product(ones, pf[rt][n], of_step[rt]);
+    }
 #pragma unroll
     for (int d = 0; d < C; ++d) {
       u32x4 vf;
@@ -345,35 +411,45 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int pair = 0; pair < 2; ++pair) {
-          if constexpr (C == 2) vf[2 * j + pair] = codes(c.v[j][0], d + 2 * pair);
-          else vf[2 * j + pair] = codes(c.v[j][pair * (C / 4) + d / 4], d % 4);
+          if constexpr (C == 2) vf[2 * j + pair] = codes<B>(c.v[j][0], d + 2 * pair, mask);
+          else vf[2 * j + pair] = codes<B>(c.v[j][pair * (C / 4) + d / 4], d % 4, mask);
         }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) o[rt][d] = product(vf, pf[rt][n], o[rt][d]);
+        for (int n = NT - 1; n >= 0; --n) o[rt][d] = product(vf, pf[rt][n], o[rt][d]);
+      // (in 32 bits sums are not left to grow by B + 8 beyond what they come to)
+      if constexpr (NT > 1) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][d] -= (B + 8.f) * of_step[rt][0];
+      }
     }
   };
 
   if (chunk_first < chunk_end) {
-    // page ids two chunks ahead, tokens one: a chunk past the end asks for the cache's first tile (no load behind a branch)
-    Chunk<HD> a, b;
-    Ids ids_a = ids_of(chunk_first), ids_b = ids_of(chunk_first + STRIDE);
-    request(chunk_first, ids_a, a);
+    // Page ids two chunks ahead, tokens one: the next chunk's keys and values take the registers of this one's as soon as these have been
+    // used.  The two ways to take a chunk are loops of their own: a branch between them would keep the sums in two places.
+    f32x4 s[RT][2];
+    Chunk<HD> c;
     int chunk = chunk_first;
-    while (true) {
-      request(chunk + STRIDE, ids_b, b);
-      Ids next = ids_of(chunk + 2 * STRIDE);
-      multiply(chunk, ids_a, a);
+    Ids ids = ids_of(chunk), next = ids_of(chunk + STRIDE);
+    request_keys(ids, c);
+    request_values(ids, c);
+    const int whole_lo = max(all_lo, lo), whole_hi = min(all_hi, hi);
+    const auto take = [&](auto whole) {
+      const Ids after = ids_of(chunk + 2 * STRIDE);
+      score(c, s);
+      request_keys(next, c);
+      add(whole, chunk, ids, c, s);
+      request_values(next, c);
       chunk += STRIDE;
-      if (chunk >= chunk_end) break;
-      ids_a = next;
-      request(chunk + STRIDE, ids_a, a);
-      next = ids_of(chunk + 2 * STRIDE);
-      multiply(chunk, ids_b, b);
-      chunk += STRIDE;
-      if (chunk >= chunk_end) break;
-      ids_b = next;
+      ids = next;
+      next = after;
+    };
+    const auto all_see = [&] { return chunk * kChunk >= whole_lo && (chunk + 1) * kChunk <= whole_hi && ids.some[0] && ids.some[1]; };
+    while (chunk < chunk_end) {
+      while (all_see()) take(std::true_type());
+      if (chunk < chunk_end) take(std::false_type());
     }
   }
 
@@ -381,16 +457,16 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] = rows_sum(l[rt]);
-    const float add = rows_sum(of_low[rt]) - 128.f * of_step[rt][0];
+    const float more = NT > 1 ? rows_sum(of_mid[rt]) : fmaf(-(B + 8.f), of_step[rt][0], rows_sum(of_mid[rt]));
 #pragma unroll
-    for (int d = 0; d < C; ++d) o[rt][d] += add;
+    for (int d = 0; d < C; ++d) o[rt][d] += more;
   }
   if constexpr (!KEYS) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (first + 16 * rt + n16 >= span.rows) continue;
       const float by = segs > 1 ? 1.f : l[rt] == 0.f ? 0.f : 1.f / l[rt];
-      float* left = segs > 1 ? scratch + ((static_cast<size_t>(row[rt]) * sh.nh + head[rt]) * max_segs + part) * (HD + 2) : nullptr;
+      float* left = segs > 1 ? scratch + ((static_cast<size_t>(row[rt]) * sh.nh + head[rt]) * sh.max_segs + part) * (HD + 2) : nullptr;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {      // lane kq has entries kq * HD / 4 on
         float x[C];
@@ -410,7 +486,10 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
       }
     }
   } else {
-    __shared__ float os[kWaves][16][HD + 4], ms[kWaves][16], ls[kWaves][16];
+    // Four waves at a time leave their sums in LDS; a row's lanes add them up, the waves in order.
+    __shared__ float os[4][16][HD + 4], ms[W][16], ls[W][16];
+    constexpr int LANES = W * kWave / 16, PER = HD / LANES > 0 ? HD / LANES : 1;      // lanes of a row, entries of a lane
+    const int r = threadIdx.x / LANES, at = threadIdx.x % LANES * PER;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (rt > 0) __syncthreads();
@@ -418,28 +497,37 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
         ms[wave][n16] = m[rt];
         ls[wave][n16] = l[rt];
       }
+      float top = -FLT_MAX, sum = 0.f, x[PER] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int turn = 0; turn < W / 4; ++turn) {
+        if (turn > 0) __syncthreads();
+        if (wave / 4 == turn) {
 #pragma unroll
-        for (int d = 0; d < C; ++d) os[wave][n16][(4 * kq + i) * C + d] = o[rt][d][i];
-      __syncthreads();
-      constexpr int LANES = kThreads / 16, PER = HD / LANES;      // lanes of a row, entries of a lane
-      const int r = threadIdx.x / LANES, at = threadIdx.x % LANES * PER, f = first + 16 * rt + r;
-      if (f >= span.rows) continue;
-      float top = ms[0][r], sum = 0.f, x[PER] = {};
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ms[w][r]);
+            for (int d = 0; d < C; ++d) os[wave % 4][n16][(4 * kq + i) * C + d] = o[rt][d][i];
+        }
+        __syncthreads();
+        if (turn == 0) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float by = __builtin_amdgcn_exp2f((ms[w][r] - top) * sh.scale_log2);
-        sum = fmaf(ls[w][r], by, sum);
+          for (int w = 0; w < W; ++w) top = fmaxf(top, ms[w][r]);
+        }
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x[e] = fmaf(os[w][r][at + e], by, x[e]);
+        for (int w = 0; w < 4; ++w) {
+          const float by = __builtin_amdgcn_exp2f((ms[4 * turn + w][r] - top) * sh.scale_log2);
+          sum = fmaf(ls[4 * turn + w][r], by, sum);
+          if (at < HD) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[e] = fmaf(os[w][r][at + e], by, x[e]);
+          }
+        }
       }
-      const size_t to = span.row0 + f / group;
-      const int h = kvh * group + f % group;
+      const int f = first + 16 * rt + r;
+      if (f >= span.rows || at >= HD) continue;
+      const int of = quotient(f, sh.group), h = kvh * group + f - of * group;
+      const size_t to = span.row0 + of;
       if (segs > 1) {
-        float* left = scratch + ((to * sh.nh + h) * max_segs + part) * (HD + 2);
+        float* left = scratch + ((to * sh.nh + h) * sh.max_segs + part) * (HD + 2);
 #pragma unroll
         for (int e = 0; e < PER; ++e) left[at + e] = x[e];
         if (at == 0) {
@@ -458,17 +546,16 @@ __global__ void __launch_bounds__(kThreads, least_waves(sizeof(T) == 4, HD, RT))
 
 // Joins the segments of a row: one wave a (row, head).
 template <class T, int HD>
-__global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ scratch, T* __restrict__ out, Rows rows, Shape sh, int max_segs) {
-  const int head = blockIdx.x, group = sh.nh / sh.nkv, lane = threadIdx.x;
+__global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ scratch, T* __restrict__ out, Rows rows, Shape sh) {
+  const int head = blockIdx.x, group = sh.group.d, lane = threadIdx.x;
   const Span span = span_of(rows, sh, blockIdx.z);
   const int at = blockIdx.y;      // position in the span
   if (at * group >= span.rows) return;
-  const int f = at * group + head % group, block_first = f / sh.tile_rows * sh.tile_rows, block_last = min(block_first + sh.tile_rows, span.rows) - 1;
-  const int block_lo = first_of(span, sh, block_first / group), block_hi = end_of(span, sh, block_last / group);
-  const int segs = block_hi > block_lo ? (block_hi - 1) / sh.segment - block_lo / sh.segment + 1 : 1;
+  const int f = at * group + head - quotient(head, sh.group) * group, block_first = f & ~(sh.tile_rows - 1);      // (tile_rows: a power of two)
+  const int segs = cut_of(span, sh, block_first, min(block_first + sh.tile_rows, span.rows) - 1).segs;
   if (segs == 1) return;
   const size_t row = span.row0 + at;
-  const float* left = scratch + (row * sh.nh + head) * max_segs * (HD + 2);
+  const float* left = scratch + (row * sh.nh + head) * sh.max_segs * (HD + 2);
   float top = -FLT_MAX;
   for (int i = 0; i < segs; ++i) top = fmaxf(top, left[i * (HD + 2) + HD]);
   constexpr int PER = (HD + kWave - 1) / kWave;
@@ -487,22 +574,26 @@ __global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ 
 
 // ---- host side
 struct Plan {
-  int rt, segment, max_segs, tile_rows, tiles;
+  int rt, waves, segment, max_segs, tile_rows, tiles;
   bool keys;
   long long floats;
 };
 
 constexpr long long kFill = 512;      // workgroups that fill the chip: two on each of 256 CUs
+constexpr int kWideChunks = 4;      // of a wave, at most, before contexts are cut
+constexpr int wide_waves(int hd) { return hd <= 64 ? 16 : 8; }      // (registers: 128 of a lane, and 256)
 
 Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
   Plan p{};
   const int group = nh / nkv;
+  max_run = std::min(max_run, T);
   const long long pairs = static_cast<long long>(max_run) * group;
   const long long waves = static_cast<long long>(units) * nkv * ((pairs + 31) / 32);
   p.keys = pairs <= 16 || waves < 2 * kFill;
   p.rt = p.keys ? (pairs > 16 && hd <= 128 ? 2 : 1) : 2;
   if (hd == 256) p.rt = 1;
-  p.tile_rows = 16 * p.rt * (p.keys ? 1 : kWaves);
+  p.waves = p.keys ? 4 : 1;
+  p.tile_rows = 16 * p.rt * (p.keys ? 1 : p.waves);
   p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
   const long long groups = static_cast<long long>(units) * nkv * p.tiles;
   const long long seen = window > 0 && window + p.tile_rows < max_context ? window + p.tile_rows : max_context;
@@ -510,9 +601,14 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   const int least = 8 * kChunk;      // tokens of a segment at least
   if (parts > (seen + least - 1) / least) parts = (seen + least - 1) / least;
   if (parts < 1) parts = 1;
+  // Few tokens: one workgroup of many waves instead of parts and a launch that joins them (32 heads over 4 of 64, one row of 529 tokens: 6.9
+  // us, with parts 8.1).
+  if (p.keys && p.rt == 1 && parts > 1 && seen <= wide_waves(hd) * kChunk * kWideChunks) {
+    parts = 1;
+    p.waves = wide_waves(hd);
+  }
   p.segment = static_cast<int>(((seen + parts - 1) / parts + least - 1) / least * least);
   if (p.segment < least) p.segment = least;
-  if (parts == 1) p.segment = 0x7FFFFFFF;
   p.max_segs = parts == 1 ? 1 : static_cast<int>((max_context + p.segment - 1) / p.segment);
   if (parts > 1 && seen < max_context) p.max_segs = static_cast<int>((seen - 1) / p.segment + 2);
   p.floats = p.max_segs == 1 ? 0 : static_cast<long long>(T) * nh * p.max_segs * (hd + 2);
@@ -530,15 +626,19 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
                what, q_stride, out_stride, window, max_context);
   KVCM_REQUIRE(rows.total > 0 && max_run > 0, "%s: %d rows, runs of up to %d", what, rows.total, max_run);
   KVCM_REQUIRE(q != nullptr && out != nullptr && cache != nullptr && tables != nullptr && rows.where != nullptr && rows.lens != nullptr, "%s: null operand", what);
+  max_run = std::min(max_run, rows.total);
   const Plan p = plan(units, rows.total, max_run, nh, nkv, hd, max_context, window);
   KVCM_REQUIRE(p.floats == 0 || (scratch != nullptr && scratch_floats >= p.floats), "%s: scratch of %lld floats is needed", what, p.floats);
-  const int page_tiles = page / kTile4;
-  Shape s{q_stride, out_stride, table_stride, nh, nkv, pages, page_tiles, -1, fabsf(scale) * 1.4426950408889634f, window,
-          static_cast<int>(static_cast<long long>(table_stride) * page < max_context ? table_stride * page : max_context), p.segment, p.tile_rows, scale < 0.f};
-  if ((page_tiles & (page_tiles - 1)) == 0) s.page_shift = __builtin_ctz(page_tiles);
+  Shape s{};
+  s.q_stride = q_stride, s.out_stride = out_stride, s.table_stride = table_stride, s.nh = nh, s.pages = pages;
+  s.max_segs = p.max_segs, s.tiles = p.tiles, s.tile_rows = p.tile_rows;
+  s.nkv = divisor(nkv), s.group = divisor(nh / nkv), s.segs = divisor(p.max_segs), s.page_tiles = divisor(page / kTile4), s.segment = divisor(p.segment / kChunk);
+  s.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  s.window = window, s.max_context = static_cast<int>(std::min<long long>(static_cast<long long>(table_stride) * page, max_context));
+  s.negate = scale < 0.f;
   if (s.scale_log2 == 0.f) s.scale_log2 = 1e-30f;      // (0 times what has not seen a token yet would not be 0)
   const long long x = static_cast<long long>(nkv) * p.max_segs * p.tiles;
-  KVCM_REQUIRE(x < (1ll << 31) && units < 65536, "%s: %lld workgroups for each of %d sequences", what, x, units);
+  KVCM_REQUIRE(x < (1ll << 30) && static_cast<long long>(rows.total) * (nh / nkv) < (1ll << 30) && units < 65536, "%s: %lld workgroups for each of %d sequences", what, x, units);
   KVCM_REQUIRE(p.max_segs == 1 || max_run < 65536, "%s: runs of %d rows cut into segments", what, max_run);
   const dim3 grid(static_cast<unsigned>(x), units);
   KVCM_HEAD4(hd, {
@@ -547,13 +647,18 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       const T* qt = static_cast<const T*>(q);
       T* ot = static_cast<T*>(out);
       const uint8_t* ct = static_cast<const uint8_t*>(cache);
-      if constexpr (HD < 256) {
-        if (p.rt == 2 && p.keys) attention4_kernel<T, HD, 2, true><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
-        if (p.rt == 2 && !p.keys) attention4_kernel<T, HD, 2, false><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
-      }
-      if (p.rt == 1 && p.keys) attention4_kernel<T, HD, 1, true><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
-      if (HD == 256 && p.rt == 1 && !p.keys) attention4_kernel<T, 256, 1, false><<<grid, kThreads, 0, stream>>>(qt, ot, ct, tables, rows, s, p.max_segs, scratch);
-      if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), kWave, 0, stream>>>(scratch, ot, rows, s, p.max_segs);
+      const auto walk = [&](auto rt, auto waves, auto keys) {
+        attention4_kernel<T, HD, decltype(rt)::value, decltype(waves)::value, decltype(keys)::value>
+            <<<grid, decltype(waves)::value * kWave, 0, stream>>>(qt, ot, ct, tables, rows, s, scratch);
+      };
+      constexpr std::integral_constant<int, 1> one;
+      constexpr std::integral_constant<int, 4> four;
+      constexpr std::integral_constant<int, HD == 256 ? 1 : 2> most;
+      if (!p.keys) walk(most, one, std::false_type());
+      else if (p.rt == 2) walk(most, four, std::true_type());
+      else if (p.waves == 4) walk(one, four, std::true_type());
+      else walk(one, std::integral_constant<int, wide_waves(HD)>(), std::true_type());
+      if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), kWave, 0, stream>>>(scratch, ot, rows, s);
     };
     if (dtype == kBF16) go(bf16_t());
     else go(float());

@@ -74,15 +74,16 @@ def attend(q, held, slots_of, visible, nh, nkv, scale, dtype):
     -> (out, tol) [rows, nh, hd]: the result in 64 bits, and how far a kernel may be from it.
 
     The tolerance, term by term (u = 2^-24, and sums of n products in 32 bits taken as 16 u of the sum of their magnitudes, what a
-    tree of matrix instructions and a walk over partial sums with a few dozen roundings stay below):
-      score      q . k is formed as step * (q . (128 + c)) + (low - 128 step) * sum q: off by e = 16 u * scale * sum|q| * (144 step + |low|)
-                 of the largest token, plus u |s| * 4 for the multiplications behind it; a score's error moves p by twice itself,
-                 and the hardware's exp2 adds 2 u |s| + 2 u
-      output     sum of p (step (128 + c)) less 128 of sum (p step), plus sum of p low: 16 u of sum p (144 step + |low|), twice for
+    tree of matrix instructions and a walk over partial sums with a few dozen roundings stay below; B = 128 for bfloat16, 16 for float;
+    mid = low + 8 step):
+      score      q . k is formed as step * (q . (B + c) - (B + 8) * sum q) + mid * sum q: off by e = 16 u * scale * sum|q| *
+                 ((B + 16) step + |mid|) of the largest token, plus u |s| * 4 for the multiplications behind it; a score's error moves p
+                 by twice itself, and the hardware's exp2 adds 2 u |s| + 2 u
+      output     sum of p step (B + c) less B + 8 of sum (p step), plus sum of p mid: 16 u of sum p ((B + 16) step + |mid|), twice for
                  the division's parts
-      bfloat16   p * step is rounded (2^-8 of it at most, what it is multiplied with is c), and so is the output (2^-8 of it)."""
+      bfloat16   p * step is rounded (2^-8 of it at most, what it is multiplied with is c - 8), and so is the output (2^-8 of it)."""
     kc, ks, kl, vc, vs, vl = held
-    u = 2.0 ** -24
+    u, w = 2.0 ** -24, 144.0 if dtype == torch.bfloat16 else 32.0
     out, tol = torch.zeros_like(q), torch.zeros_like(q)
     for r in range(q.shape[0]):
         first, end = visible[r]
@@ -95,9 +96,10 @@ def attend(q, held, slots_of, visible, nh, nkv, scale, dtype):
             x = (k @ q[r, h]) * scale
             p = torch.softmax(x, 0)
             out[r, h] = p @ v
-            e = 16 * u * abs(scale) * q[r, h].abs().sum() * (144 * ks[s, g] + kl[s, g].abs()).max() + 8 * u * x.abs().max() + 4 * u
-            t = 2 * e * (p @ (v - out[r, h]).abs()) + 2 * 16 * u * (p @ (144 * vs[s, g] + vl[s, g].abs() + 0 * v))
+            k_mid, v_mid = (kl[s, g] + 8 * ks[s, g]).abs(), (vl[s, g] + 8 * vs[s, g]).abs()
+            e = 16 * u * abs(scale) * q[r, h].abs().sum() * (w * ks[s, g] + k_mid).max() + 8 * u * x.abs().max() + 4 * u
+            t = 2 * e * (p @ (v - out[r, h]).abs()) + 2 * 16 * u * (p @ (w * vs[s, g] + v_mid + 0 * v))
             if dtype == torch.bfloat16:
-                t = t + 2.0 ** -8 * (p @ (vs[s, g] * vc[s, g])) + 2.0 ** -8 * out[r, h].abs()
+                t = t + 2.0 ** -8 * (p @ (vs[s, g] * (vc[s, g] - 8).abs())) + 2.0 ** -8 * out[r, h].abs()
             tol[r, h] = t
     return out, tol
