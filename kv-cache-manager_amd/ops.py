@@ -3,6 +3,7 @@ the host that their shapes and dtypes are what the kernel assumes, and launches 
 current stream.  There is no fallback: without the library (or without a GPU) these raise.
 """
 import ctypes as C
+import functools
 import os
 import struct as _struct
 import sys
@@ -1231,21 +1232,29 @@ def cache4_shape(pages, nkv, hd, block_size=16):
     return (pages, nkv, block_size // 16, 16 * (hd + 8))
 
 
+# (What follows runs before every launch of a few microseconds: a tensor is asked once for what is needed of it, and a message is made only
+# when it is needed.)
 def _one_gpu(*ts):
-    """Launches go to device 0's current stream: every operand lives there, and it is the current device."""
+    """The operands' addresses (None: 0).  Launches go to device 0's current stream: every operand lives there, and it is the current device."""
+    at = []
     for t in ts:
-        if t is not None and t.get_device() != 0:
+        if t is None:
+            at.append(0)
+        elif t.get_device():
             _dev(t)
             raise ValueError("kernel operands must live on device 0")
-    if torch._C._cuda_getDevice() != 0:
+        else:
+            at.append(t.data_ptr())
+    if torch._C._cuda_getDevice():
         raise ValueError("device 0 must be the current device")
+    return at
 
 
-# (These checks run before every launch; a message is made only when it is needed: one made on every call costs as much as the check.)
-def _check_cache4(cache, nkv, hd, nh=None):
+def _check_cache4(cache, at, nkv, hd, nh=None):
+    """-> pages, tokens of a page."""
     s = cache.shape
-    if not (cache.dtype == torch.uint8 and len(s) == 4 and s[1] == nkv > 0 and hd in _HEADS4 and s[3] == 16 * (hd + 8) and s[0] > 0 and s[2] > 0
-            and cache.is_contiguous() and cache.data_ptr() % 16 == 0):
+    if not (len(s) == 4 and s[1] == nkv > 0 and hd in _HEADS4 and s[3] == 16 * (hd + 8) and cache.dtype is torch.uint8 and cache.is_contiguous()
+            and s[0] > 0 and s[2] > 0 and at % 16 == 0):
         raise ValueError("the cache must be contiguous uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)], aligned to 16 bytes (cache4_shape)")
     if s[0] * s[2] >= 2 ** 27:
         raise ValueError("a cache of 2^31 token slots or more does not fit 32-bit slot numbers")
@@ -1254,13 +1263,13 @@ def _check_cache4(cache, nkv, hd, nh=None):
     return s[0], 16 * s[2]
 
 
-def _long_rows(t, name, rows, cols, dtype=None):
+def _long_rows(t, name, rows, cols, dtype):
     """The stride of a matrix of rows (a single row's may be anything)."""
     s, st = t.shape, t.stride()
     if len(s) != 2 or (st[1] != 1 and s[1] > 1):
         raise ValueError(f"{name} must be 2-d with unit inner stride")
-    if t.dtype not in _DT or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name} must be {'bfloat16 or float32' if dtype is None else dtype}")
+    if t.dtype is not dtype or dtype not in _DT:
+        raise ValueError(f"{name} must be {dtype if dtype in _DT else 'bfloat16 or float32'}")
     if not (s[0] >= rows >= 0 and s[1] >= cols and (st[0] >= cols or rows <= 1) and st[0] < 2 ** 31):
         raise ValueError(f"{name} must be [>= {rows}, >= {cols}] with rows of their own")
     return max(st[0], cols)
@@ -1272,48 +1281,54 @@ def rope_cache4(qkv, nh, nkv, hd, cache, slots, cos_sin=None, q_out=None, rows=N
     [rows, hd/2, 2]) k is rotated before, as ``rope_cache`` does, and q as well, to ``q_out`` [rows, nh * hd] (default: in its place
     in ``qkv``); k and v of ``qkv`` stay as they are.  Without it nothing is rotated and q is not touched."""
     T = qkv.shape[0] if rows is None else rows
-    _one_gpu(qkv, cache, slots, cos_sin, q_out)
-    pages, page = _check_cache4(cache, nkv, hd, nh)
-    stride = _long_rows(qkv, "qkv", T, (nh + 2 * nkv) * hd)
+    at, cache_at, slots_at, table_at, q_at = _one_gpu(qkv, cache, slots, cos_sin, q_out)
+    pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
+    dtype = qkv.dtype
+    stride = _long_rows(qkv, "qkv", T, (nh + 2 * nkv) * hd, dtype)
     _i32(slots, "slots", T)
-    _need(cos_sin is not None or q_out is None, "q_out is for rotated queries: cos_sin is missing")
     q_stride = 0
-    if cos_sin is not None:
-        _need(cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.numel() >= T * hd and cos_sin.data_ptr() % 16 == 0,
-              "cos_sin must be float32 [rows, head_dim/2, 2], aligned to 16 bytes")
-        q_out = qkv if q_out is None else q_out
-        q_stride = _long_rows(q_out, "q_out", T, nh * hd, qkv.dtype)
-    _call("kvcm_rope_cache4", _ptr(qkv), _DT[qkv.dtype], stride, _ptr(q_out), q_stride, _ptr(cache), _ptr(slots), _ptr(cos_sin), T, nh, nkv, hd,
-          pages, page, _stream())
+    if cos_sin is None:
+        _need(q_out is None, "q_out is for rotated queries: cos_sin is missing")
+    else:
+        if not (cos_sin.dtype is torch.float32 and cos_sin.is_contiguous() and cos_sin.numel() >= T * hd and table_at % 16 == 0):
+            raise ValueError("cos_sin must be float32 [rows, head_dim/2, 2], aligned to 16 bytes")
+        if q_out is None:
+            q_at, q_stride = at, stride
+        else:
+            q_stride = _long_rows(q_out, "q_out", T, nh * hd, dtype)
+    _call("kvcm_rope_cache4", at, _DT[dtype], stride, q_at, q_stride, cache_at, slots_at, table_at, T, nh, nkv, hd, pages, page, _stream())
 
 
 def cache4_rows(cache, slots, k, v, rows=None):
     """Reads the tokens at ``slots`` back from a 4-bit cache: k, v [rows, nkv * hd] (bfloat16 or float32, both alike).  A slot outside the
     pages (-1) gives zeros."""
     n = slots.numel() if rows is None else rows
-    _one_gpu(cache, slots, k, v)
-    _need(cache.dim() == 4, "the cache must be uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)] (cache4_shape)")
-    nkv, hd = cache.shape[1], cache.shape[3] // 16 - 8
-    pages, page = _check_cache4(cache, nkv, hd)
+    cache_at, slots_at, k_at, v_at = _one_gpu(cache, slots, k, v)
+    s = cache.shape
+    _need(len(s) == 4, "the cache must be uint8 [pages, nkv, block_size / 16, 16 * (hd + 8)] (cache4_shape)")
+    nkv, hd = s[1], s[3] // 16 - 8
+    pages, page = _check_cache4(cache, cache_at, nkv, hd)
     _i32(slots, "slots", n)
-    k_stride, v_stride = _long_rows(k, "k", n, nkv * hd), _long_rows(v, "v", n, nkv * hd, k.dtype)
-    _call("kvcm_cache4_rows", _ptr(cache), _ptr(slots), _ptr(k), k_stride, _ptr(v), v_stride, _DT[k.dtype], n, nkv, hd, pages, page, _stream())
+    dtype, cols = k.dtype, nkv * hd
+    k_stride, v_stride = _long_rows(k, "k", n, cols, dtype), _long_rows(v, "v", n, cols, dtype)
+    _call("kvcm_cache4_rows", cache_at, slots_at, k_at, k_stride, v_at, v_stride, _DT[dtype], n, nkv, hd, pages, page, _stream())
 
 
 def _scratch4(what, need, scratch, device):
+    """Scratch and its floats."""
     if scratch is None:
-        if not need:
-            return None
         if _recording is not None:
             raise ValueError(f"{what}: a recorded step must bring its scratch (an allocation here would not outlive the step)")
-        return torch.empty(need, dtype=torch.float32, device=device)
-    if scratch.dtype != torch.float32 or not scratch.is_contiguous():
+        return torch.empty(need, dtype=torch.float32, device=device), need
+    if scratch.dtype is not torch.float32 or not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous float32")
-    if scratch.numel() < need:
+    n = scratch.numel()
+    if n < need:
         raise ValueError(f"{what}: scratch of {need} floats is needed")
-    return scratch
+    return scratch, n
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_decode4_scratch(rows, nh, nkv, hd, max_context, window=0):
     """Floats of scratch ``attention_decode4`` needs for these sizes (0: contexts are not cut)."""
     return int(lib().kvcm_attention_decode4_scratch(rows, nh, nkv, hd, int(max_context), int(window)))
@@ -1326,19 +1341,27 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
     no page hides its tokens.  ``max_context`` bounds every row's context length and decides how contexts are cut into parts that run side
     by side, which needs ``scratch`` (attention_decode4_scratch floats; allocated here when not given)."""
     T = q.shape[0] if rows is None else rows
-    _one_gpu(q, out, cache, tables, row_seq, ctx_lens, scratch)
-    pages, page = _check_cache4(cache, nkv, hd, nh)
-    q_stride, out_stride = _long_rows(q, "q", T, nh * hd), _long_rows(out, "out", T, nh * hd, q.dtype)
-    for t, name, n in ((row_seq, "row_seq", T), (ctx_lens, "ctx_lens", T), (tables, "tables", 1)):
-        _i32(t, name, n)
-    _need(table_stride > 0 and tables.numel() >= table_stride, "tables must hold rows of table_stride pages")
-    _need(window >= 0 and max_context >= 0, "window and max_context must not be negative")
-    scratch = _scratch4("attention_decode4", attention_decode4_scratch(T, nh, nkv, hd, max_context, window), scratch, q.device)
-    _call("kvcm_attention_decode4", _ptr(q), _DT[q.dtype], q_stride, _ptr(out), out_stride, _ptr(cache), _ptr(tables), table_stride,
-          tables.numel() // table_stride, _ptr(row_seq), _ptr(ctx_lens), T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context),
-          _ptr(scratch), scratch.numel() if scratch is not None else 0, _stream())
+    q_at, out_at, cache_at, tables_at, seq_at, lens_at, scratch_at = _one_gpu(q, out, cache, tables, row_seq, ctx_lens, scratch)
+    pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
+    dtype, cols = q.dtype, nh * hd
+    q_stride, out_stride = _long_rows(q, "q", T, cols, dtype), _long_rows(out, "out", T, cols, dtype)
+    _i32(row_seq, "row_seq", T)
+    _i32(ctx_lens, "ctx_lens", T)
+    held = tables.numel()
+    _i32(tables, "tables")
+    if not held >= table_stride > 0:
+        raise ValueError("tables must hold rows of table_stride pages")
+    if window < 0 or max_context < 0:
+        raise ValueError("window and max_context must not be negative")
+    need, floats = attention_decode4_scratch(T, nh, nkv, hd, max_context, window), 0
+    if need or scratch is not None:
+        scratch, floats = _scratch4("attention_decode4", need, scratch, q.device)
+        scratch_at = scratch.data_ptr()
+    _call("kvcm_attention_decode4", q_at, _DT[dtype], q_stride, out_at, out_stride, cache_at, tables_at, table_stride, held // table_stride, seq_at,
+          lens_at, T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context), scratch_at, floats, _stream())
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_prefill4_scratch(rows, nh, nkv, hd, max_context, max_run, num_seqs, window=0):
     """Floats of scratch ``attention_prefill4`` needs for a launch of these sizes (0: contexts are not cut)."""
     return int(lib().kvcm_attention_prefill4_scratch(rows, nh, nkv, hd, int(max_context), max_run, num_seqs, int(window)))
@@ -1351,18 +1374,24 @@ def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start
     tokens up to its own position (``window`` > 0: the last ``window`` of them).  Rows of no run are left as they are.
     ``max_context``: a bound of every row's context length (default: what the tables can hold)."""
     T = q.shape[0] if rows is None else rows
-    _one_gpu(q, out, cache, tables, run_start, seq_start, scratch)
-    pages, page = _check_cache4(cache, nkv, hd, nh)
-    q_stride, out_stride = _long_rows(q, "q", T, nh * hd), _long_rows(out, "out", T, nh * hd, q.dtype)
-    _need(table_stride > 0 and num_seqs >= 0 and max_run >= 0 and window >= 0, "table_stride must be positive, num_seqs, max_run and window not negative")
-    for t, name, n in ((run_start, "run_start", num_seqs + 1), (seq_start, "seq_start", num_seqs), (tables, "tables", num_seqs * table_stride)):
-        _i32(t, name, n)
+    q_at, out_at, cache_at, tables_at, run_at, start_at, scratch_at = _one_gpu(q, out, cache, tables, run_start, seq_start, scratch)
+    pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
+    dtype, cols = q.dtype, nh * hd
+    q_stride, out_stride = _long_rows(q, "q", T, cols, dtype), _long_rows(out, "out", T, cols, dtype)
+    if table_stride <= 0 or num_seqs < 0 or max_run < 0 or window < 0:
+        raise ValueError("table_stride must be positive, num_seqs, max_run and window not negative")
+    _i32(run_start, "run_start", num_seqs + 1)
+    _i32(seq_start, "seq_start", num_seqs)
+    _i32(tables, "tables", num_seqs * table_stride)
     max_context = table_stride * page if max_context is None else max_context
-    _need(max_context >= 0, "max_context must not be negative")
-    scratch = _scratch4("attention_prefill4", attention_prefill4_scratch(T, nh, nkv, hd, max_context, max_run, num_seqs, window), scratch, q.device)
-    _call("kvcm_attention_prefill4", _ptr(q), _DT[q.dtype], q_stride, _ptr(out), out_stride, _ptr(cache), _ptr(tables), table_stride, _ptr(run_start),
-          _ptr(seq_start), num_seqs, max_run, T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context), _ptr(scratch),
-          scratch.numel() if scratch is not None else 0, _stream())
+    if max_context < 0:
+        raise ValueError("max_context must not be negative")
+    need, floats = attention_prefill4_scratch(T, nh, nkv, hd, max_context, max_run, num_seqs, window), 0
+    if need or scratch is not None:
+        scratch, floats = _scratch4("attention_prefill4", need, scratch, q.device)
+        scratch_at = scratch.data_ptr()
+    _call("kvcm_attention_prefill4", q_at, _DT[dtype], q_stride, out_at, out_stride, cache_at, tables_at, table_stride, run_at, start_at, num_seqs, max_run,
+          T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context), scratch_at, floats, _stream())
 
 
 # ------------------------------------------------------------------------- probes of the machine
