@@ -98,19 +98,6 @@ struct Rows {
   bool runs;
 };
 
-// Division by a number that the host knows: a single token's walk is a few microseconds long, and dividing by a variable takes some
-// twenty instructions each time.  n / d = 2 n * by / 2^32 / 2^shift with by = 2^(31 + shift) / d rounded up, shift = log2 d rounded down:
-// too much by less than n / 2^(31 + shift) * d / d, below 1 / d for n < 2^30.
-struct Divisor {
-  int d, shift;
-  unsigned by;
-};
-inline Divisor divisor(int d) {
-  const int shift = 31 - __builtin_clz(d);
-  return Divisor{d, shift, static_cast<unsigned>(((1ull << (31 + shift)) + d - 1) / d)};
-}
-__device__ __forceinline__ int quotient(int n, const Divisor& d) { return static_cast<int>(__umulhi(2u * n, d.by) >> d.shift); }
-
 struct Shape {
   int q_stride, out_stride, table_stride, nh, pages, max_segs, tiles;
   Divisor nkv, group, segs, page_tiles, segment;      // segment: in chunks (and max_segs 1: not looked at)

@@ -40,6 +40,19 @@ __device__ __forceinline__ int value4_byte(int t, int u) {
 __device__ __forceinline__ float step4(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float low4(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
 
+// Division by a number that the host knows: these kernels are a few microseconds long, and dividing by a variable takes some twenty
+// instructions each time.  n / d = 2 n * by / 2^32 / 2^shift with by = 2^(31 + shift) / d rounded up, shift = log2 d rounded down: too much
+// by less than n / 2^(31 + shift) * d / d, below 1 / d for n < 2^30.
+struct Divisor {
+  int d, shift;
+  unsigned by;
+};
+inline Divisor divisor(int d) {
+  const int shift = 31 - __builtin_clz(d);
+  return Divisor{d, shift, static_cast<unsigned>(((1ull << (31 + shift)) + d - 1) / d)};
+}
+__device__ __forceinline__ int quotient(int n, const Divisor& d) { return static_cast<int>(__umulhi(2u * n, d.by) >> d.shift); }
+
 inline bool head4(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
 
 }  // namespace kvcm

@@ -14,11 +14,11 @@ def bf16_bits(x):
 def encode(x):
     """One vector -> (codes, step, low); low is never -0."""
     x = np.asarray(x, dtype=np.float64)
-    if not np.isfinite(x).all():
+    if not np.isfinite(x).all() or abs(x.max() - bf16(x.min())) > np.finfo(np.float32).max:
         return np.zeros(len(x), dtype=int), float("nan"), float(bf16(np.nanmin(x)))
     low = float(bf16(x.min())) + 0.0
     step = float(bf16(np.float32((x.max() - low) / 15.0)))
-    if step == 0.0:
+    if step <= 0.0:      # (below 0: low was rounded above the highest entry)
         return np.zeros(len(x), dtype=int), 0.0, low
     return np.clip(np.rint((x - low) / step), 0, 15).astype(int), step, low
 

@@ -57,7 +57,11 @@ def test_store_writes_the_format_and_nothing_else(ops, nh, nkv, hd, page, rotate
     rows[4] = 1.5                                        # no range: step 0
     rows[5, ::3] = 2.0 ** -130                           # ranges of denormal steps
     rows[6] *= 1e30
+    rows[15] = 1.005                                     # float rows: no range, and low is rounded above it
+    rows[16] = 1.001                                     # and below it
     if not rotate:
+        rows[17, nh * hd] = 3e38                         # a range that passes the largest float
+        rows[17, nh * hd + 1] = -3e38
         rows[7, nh * hd + 1] = float("inf")
         rows[8, -1] = float("nan")
         rows[9, -hd:] = float("-inf")
