@@ -10,24 +10,27 @@
 //
 // Codes become operands without arithmetic: in bfloat16 0x4300 | c is 128 + c and 0x4180 | c << 3 is 16 + c, exactly, and one shift and one
 // bit operation give two of them (7 or 8 instructions for 8 codes; keys and values both lie in the order that this needs).  Rows of
-// bfloat16 take B = 128, float rows, whose 32 bits the larger numbers would eat into, B = 16.  With k = mid + step (c - 8), where mid =
-// low + 8 step is the middle of a vector's range,
-//   q . k = step (q . (B + c) - (B + 8) sum q) + mid sum q         the sum of a row's q once, -(B + 8) times it as the accumulator's start
-//   sum p v = sum (p step) (B + c) - (B + 8) sum (p step) + sum p mid
+// bfloat16 take B = 128, float rows, whose 32 bits the larger numbers would eat into, B = 16.  With f the scale times log2 e,
+//   f q . k - m = (f step) (q . (B + c)) + [low (f sum q) - B step (f sum q) - m]
+// where the bracket is a matrix instruction of its own, m its accumulator's start: a pair (step, low) as it lies in the cache is an
+// operand, against f sum q as three bfloat16 numbers (24 bits) and -B times them.  (Float rows: q . (B + c) - (B + 8) sum q comes first,
+// the small terms of q before the large, and 8 step in the bracket: sums stay as small as what they come to.)  One multiplication and
+// addition for each score leaves the exponential's argument.
+//   sum p v = sum (p step) (B + c) - (B + 8) sum (p step) + sum p (low + 8 step)
 // where p step is what is rounded to bfloat16 (float rows: split into three, which keep all 24 bits, as q is), and its sum comes from
 // one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0
-// as the values are from their middle.  sum p and sum p mid stay in 32 bits.
+// as the values are from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
 //
-// How the work is laid out (a rule on sizes, `plan`):
-//   KEYS   the waves of a workgroup share a tile of rows and take every W-th 32 tokens; their m, l, o meet in LDS.  For single
-//          tokens and short runs: their time is reading the cache.
-//   rows   a wave has rows of its own.  For runs of many rows: vector instructions bound it (some 120 of a wave for 16 rows and 32
-//          tokens of 64 entries beside 9 matrix instructions).
-// and contexts are cut into segments that run as workgroups of their own while there are few; a second launch joins what they leave
+// m is not the largest score but one that no score passes by more than 2^6: it moves in few chunks, and only then do a row's four lanes
+// compare what they have and the sums get scaled.
+//
+// How the work is laid out (a rule on sizes, `plan`): the W waves of a workgroup share a tile of rows and take every W-th 32 tokens; their m, l, o
+// meet in LDS.  Single tokens are bound by reading the cache, runs of many rows by vector instructions (some 250 of a wave for 32 rows and 32
+// tokens of 128 entries, beside 38 matrix instructions).  Waves with rows of their own walk four times as long, and the last of them
+// alone: 446 us instead of 285 for portions of prompts behind contexts of 3,000 to 8,000 tokens (32 heads over 8 of 128); with operands that four such
+// waves make for one another in LDS, a quarter fewer instructions and a barrier every 64 tokens, 475 us.
+// Contexts are cut into segments that run as workgroups of their own while there are few; a second launch joins what they leave
 // in scratch (o, m, l in 32 bits, in the order of the segments).
-//
-// The maximum m that a row's exponentials are taken against is not the largest score but one that no score passes by more than 2^6: it
-// moves in few chunks, and only then do a row's four lanes compare what they have and the sums get scaled.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -46,7 +49,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 32;      // tokens a wave takes at a time: two tiles of the cache
-constexpr float kAhead = 6.f;   // the maximum that a row's exponentials are taken against follows when a score is 2^6 ahead of it
+constexpr float kAhead = 6.f;   // m follows when a score is 2^6 ahead of it
 
 __device__ __forceinline__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2)); }
 __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
@@ -84,11 +87,13 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// What a lane holds of 32 tokens: of either tile, a key's HD / 4 codes, four tokens' HD / 16 value codes, and the pairs of these four.
+// What a lane holds of 32 tokens: of either tile, a key's HD / 4 codes, four tokens' HD / 16 value codes, and the pairs of
+// these four.
 template <int HD>
 struct Chunk {
   uint32_t k[2][HD / 32], v[2][HD / 32];
   u32x4 kp[2], vp[2];
+  uint32_t of_token[2];      // the pair of token lane % 16's key
 };
 
 // Where rows come from: single tokens (where = row_seq, lens = ctx_lens) or runs (run_start, seq_start).
@@ -103,7 +108,6 @@ struct Shape {
   Divisor nkv, group, segs, page_tiles, segment;      // segment: in chunks (and max_segs 1: not looked at)
   float scale_log2;
   int window, max_context, tile_rows;
-  bool negate;      // a negative scale: of the queries
 };
 
 struct Span {
@@ -165,12 +169,18 @@ __device__ __forceinline__ void store_some(T* p, const float (&x)[N]) {
   }
 }
 
+__device__ __forceinline__ uint32_t in_vector_register(uint32_t x) {
+  uint32_t r;
+  asm("v_mov_b32 %0, %1" : "=v"(r) : "s"(x));
+  return r;
+}
+
 // blockIdx.x: kv head (fastest: with eight of them each of the chip's eight parts keeps to one), then segment, then tile of rows, the last
 // tile first (it sees the most keys); blockIdx.y: token or sequence.
 constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what the registers are bounded for
   return hd == 256 ? 1 : wide ? (rt == 1 ? 2 : 1) : hd == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 2;
 }
-template <class T, int HD, int RT, int W, bool KEYS>
+template <class T, int HD, int RT, int W>
 __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
                                                               const int* __restrict__ tables, Rows rows, Shape sh, float* __restrict__ scratch) {
   constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>, B = kBias<T>;
@@ -178,44 +188,35 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, n16 = lane % 16, kq = lane / 16;
   const int group = sh.group.d;
   const Span span = span_of(rows, sh, blockIdx.y);
-  const int block_first = (sh.tiles - 1 - tile_up) * sh.tile_rows;      // of the span's pairs
-  if (block_first >= span.rows) return;
-  const int block_last = min(block_first + sh.tile_rows, span.rows) - 1;
+  const int first = (sh.tiles - 1 - tile_up) * sh.tile_rows;      // of the span's pairs
+  if (first >= span.rows) return;
+  const int last = min(first + sh.tile_rows, span.rows) - 1;
   // the workgroup's tokens, and the segment of them that it takes
-  const Cut cut = cut_of(span, sh, block_first, block_last);
+  const Cut cut = cut_of(span, sh, first, last);
   const int segs = cut.segs;
   if (part >= segs) return;
-  const int first = block_first + (KEYS ? 0 : wave * 16 * RT);
-  const int last = min(first + 16 * RT, span.rows) - 1;
-  if (!KEYS && first > block_last) return;      // (no barriers where waves have rows of their own)
   const int seg_first = sh.max_segs == 1 ? 0 : (cut.first + part) * sh.segment.d * kChunk;
   const int seg_end = sh.max_segs == 1 ? 0x7FFFFFFF : static_cast<int>(min(0x7FFFFFFFu, static_cast<unsigned>(seg_first) + sh.segment.d * kChunk));
   const int at_first = quotient(first, sh.group), at_last = quotient(last, sh.group);
   const int lo = max(first_of(span, sh, at_first), seg_first), hi = min(end_of(span, sh, at_last), seg_end);
-  const int all_lo = first_of(span, sh, at_last), all_hi = end_of(span, sh, at_first);      // what every row of the wave sees
+  const int all_lo = first_of(span, sh, at_last), all_hi = end_of(span, sh, at_first);      // what every row sees
 
-  int row[RT], head[RT], row_lo[RT], row_hi[RT];
-  float q_sum[RT];
+  int row_lo[RT], row_hi[RT];
+  u32x4 qf[RT][NT][KS], q_sum[RT];
   f32x4 start[RT];
-  u32x4 qf[RT][NT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int f = min(first + 16 * rt + n16, span.rows - 1);      // pairs past the end repeat the last one; they are never stored
-    const int at = quotient(f, sh.group);
-    row[rt] = span.row0 + at;
-    head[rt] = kvh * group + f - at * group;
+    const int at = quotient(f, sh.group), head = kvh * group + f - at * group;
     row_lo[rt] = max(first_of(span, sh, at), seg_first);
     row_hi[rt] = min(end_of(span, sh, at), seg_end);
     float sum = 0.f;
 #pragma unroll
     for (int c = 0; c < KS; ++c) {
       float x[8];
-      load_eight(q + static_cast<size_t>(row[rt]) * sh.q_stride + head[rt] * HD + kq * (HD / 4) + 8 * c, x);
+      load_eight(q + static_cast<size_t>(span.row0 + at) * sh.q_stride + head * HD + kq * (HD / 4) + 8 * c, x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = sh.negate ? -x[i] : x[i];
-        sum += x[i];
-      }
+      for (int i = 0; i < 8; ++i) sum += x[i];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -227,29 +228,35 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
           }
         }
     }
-    q_sum[rt] = rows_sum(sum);
-    const float less = -(B + 8.f) * q_sum[rt];
-    start[rt] = f32x4{less, less, less, less};
+    sum = rows_sum(sum);
+    const float less = -(B + 8.f) * sum;
+    start[rt] = f32x4{less, less, less, less};      // (float rows)
+    // against a pair (step, low), three times: what step and low are multiplied with (the first lane of a row; the others' is 0)
+    float left = kq == 0 ? sum * sh.scale_log2 : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float term = i < 3 ? round_to<bf16_t>(left) : 0.f;
+      q_sum[rt][i] = pack((NT == 1 ? -B : 8.f) * term, term);
+      left -= term;
+    }
   }
 
-  float m[RT], l[RT], of_mid[RT];
-  f32x4 o[RT][C], of_step[RT];
+  float limit[RT], l[RT], of_mid[RT];      // limit: how far ahead of m a score may be (-FLT_MAX: no score yet, and m is 0)
+  f32x4 less_m[RT], o[RT][C], of_step[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -FLT_MAX;
+    limit[rt] = -FLT_MAX;
     l[rt] = of_mid[rt] = 0.f;
-    of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    less_m[rt] = of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < C; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  constexpr int STRIDE = KEYS ? W : 1;
-  const int chunk_first = lo / kChunk + (KEYS ? wave : 0), chunk_end = (hi + kChunk - 1) / kChunk;      // every STRIDE-th of them
+  const int chunk_first = lo / kChunk + wave, chunk_end = (hi + kChunk - 1) / kChunk;      // every W-th of them
   const int* table = tables + static_cast<size_t>(max(span.seq, 0)) * sh.table_stride;      // (looked at only where there are tokens)
   const int k_at = n16 * (HD / 2) + kq * (HD / 8), v_at = value4_at(HD) + (kq * 16 + n16) * (HD / 8);
-  const int kp_at = 8 * HD + kq * 16, vp_at = value4_at(HD) + 8 * HD + kq * 16;
-  uint32_t mask;
-  asm("v_mov_b32 %0, %1" : "=v"(mask) : "n"(kMask<B>));
+  const int kp_at = 8 * HD + kq * 16, vp_at = value4_at(HD) + 8 * HD + kq * 16, token_at = 8 * HD + n16 * 4;
+  const uint32_t mask = in_vector_register(kMask<B>);
 
   // Of either tile of a chunk: where it lies, and whether it has tokens.  One past the end stands for the last, one whose page is none for
   // the cache's first page (nobody looks at their tokens): no load and no address is behind a branch.
@@ -275,6 +282,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
       const uint8_t* p = cache + ids.at[j];
       load_words(p + k_at, c.k[j]);
       c.kp[j] = *reinterpret_cast<const u32x4*>(p + kp_at);
+      c.of_token[j] = *reinterpret_cast<const uint32_t*>(p + token_at);
     }
   };
   auto request_values = [&](const Ids& ids, Chunk<HD>& c) {
@@ -286,77 +294,75 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     }
   };
 
+  // s = scale * log2 e * q . k - m
   auto score = [&](const Chunk<HD>& c, f32x4 (&s)[RT][2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       u32x4 kf[KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) kf[k] = u32x4{codes<B>(c.k[j][k], 0, mask), codes<B>(c.k[j][k], 1, mask), codes<B>(c.k[j][k], 2, mask), codes<B>(c.k[j][k], 3, mask)};
-      if constexpr (NT == 1) {
+      const u32x4 pairs{c.of_token[j], c.of_token[j], c.of_token[j], c.of_token[j]};
+      float step[4];
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+      for (int i = 0; i < 4; ++i) step[i] = step4(c.kp[j][i]) * sh.scale_log2;
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][j] = product(kf[k], qf[rt][0][k], k == 0 ? start[rt] : s[rt][j]);
-      } else {
-        // 32 bits are to be kept: the small terms first, by themselves
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          s[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int rt = 0; rt < RT; ++rt) {
+        const f32x4 rest = product(pairs, q_sum[rt], less_m[rt]);
+        f32x4 x{0.f, 0.f, 0.f, 0.f};
+        if constexpr (NT > 1) {
 #pragma unroll
           for (int n = NT - 1; n > 0; --n)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) s[rt][j] = product(kf[k], qf[rt][n][k], s[rt][j]);
-          s[rt][j] += start[rt];
-#pragma unroll
-          for (int k = 0; k < KS; ++k) s[rt][j] = product(kf[k], qf[rt][0][k], s[rt][j]);
+            for (int k = 0; k < KS; ++k) x = product(kf[k], qf[rt][n][k], x);
+          x += start[rt];
         }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) x = product(kf[k], qf[rt][0][k], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[rt][j][i] = fmaf(step[i], x[i], rest[i]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float step = step4(c.kp[j][i]), mid = fmaf(8.f, step, low4(c.kp[j][i]));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][j][i] = fmaf(step, s[rt][j][i], mid * q_sum[rt]);
-      }
   };
   // WHOLE: every row sees all 32 tokens
   auto add = [&](auto whole, int chunk, const Ids& ids, const Chunk<HD>& c, f32x4 (&s)[RT][2]) {
     constexpr bool WHOLE = decltype(whole)::value;
     bool ok[RT][2][4];
-    float mx[RT];
+    float top[RT];
     bool move = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      mx[rt] = -FLT_MAX;
+      top[rt] = -FLT_MAX;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = chunk * kChunk + 16 * j + 4 * kq + i;
-          ok[rt][j][i] = WHOLE || ((t >= row_lo[rt]) & (t < row_hi[rt]) & (ids.some[j]));
+          ok[rt][j][i] = WHOLE || ((t >= row_lo[rt]) & (t < row_hi[rt]) & ids.some[j]);
           s[rt][j][i] = ok[rt][j][i] ? s[rt][j][i] : -FLT_MAX;
-          mx[rt] = fmaxf(mx[rt], s[rt][j][i]);
+          top[rt] = fmaxf(top[rt], s[rt][j][i]);
         }
-      move |= (mx[rt] - m[rt]) * sh.scale_log2 > kAhead;
+      move |= top[rt] > limit[rt];
     }
     if (__builtin_amdgcn_ballot_w64(move)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float top = fmaxf(m[rt], rows_max(mx[rt])), alpha = __builtin_amdgcn_exp2f((m[rt] - top) * sh.scale_log2);
-        m[rt] = top;
+        const float most = rows_max(top[rt]);
+        const bool moves = most > limit[rt];
+        const float by = moves ? most : 0.f, alpha = limit[rt] == -FLT_MAX ? 1.f : __builtin_amdgcn_exp2f(-by);      // (no score yet: nothing to scale)
+        limit[rt] = moves ? kAhead : limit[rt];
+        less_m[rt] -= by;
         l[rt] *= alpha;
         of_mid[rt] *= alpha;
         of_step[rt] *= alpha;
 #pragma unroll
         for (int d = 0; d < C; ++d) o[rt][d] *= alpha;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[rt][j] -= by;
       }
     }
     u32x4 pf[RT][NT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float shift = -m[rt] * sh.scale_log2;
       float p_step[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -364,9 +370,8 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
         for (int i = 0; i < 4; ++i) {
           // zero times what a place that is not seen holds (an Inf, a NaN) would not be zero
           const uint32_t pair = ok[rt][j][i] ? c.vp[j][i] : 0u;
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[rt][j][i], sh.scale_log2, shift)), p = ok[rt][j][i] ? e : 0.f;
+          const float e = __builtin_amdgcn_exp2f(s[rt][j][i]), p = ok[rt][j][i] ? e : 0.f, step = step4(pair);
           l[rt] += p;
-          const float step = step4(pair);
           of_mid[rt] = fmaf(p, fmaf(8.f, step, low4(pair)), of_mid[rt]);
           p_step[j][i] = p * step;
         }
@@ -419,17 +424,17 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     f32x4 s[RT][2];
     Chunk<HD> c;
     int chunk = chunk_first;
-    Ids ids = ids_of(chunk), next = ids_of(chunk + STRIDE);
+    Ids ids = ids_of(chunk), next = ids_of(chunk + W);
     request_keys(ids, c);
     request_values(ids, c);
     const int whole_lo = max(all_lo, lo), whole_hi = min(all_hi, hi);
     const auto take = [&](auto whole) {
-      const Ids after = ids_of(chunk + 2 * STRIDE);
+      const Ids after = ids_of(chunk + 2 * W);
       score(c, s);
       request_keys(next, c);
       add(whole, chunk, ids, c, s);
       request_values(next, c);
-      chunk += STRIDE;
+      chunk += W;
       ids = next;
       next = after;
     };
@@ -440,93 +445,60 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     }
   }
 
-  // o / l of a wave's rows, or (o, m, l) where waves or segments still have to be joined
+  // Four waves at a time leave their sums in LDS; a row's lanes add them up, the waves in order.
+  __shared__ float os[4][16][HD + 4], ms[W][16], ls[W][16];
+  constexpr int LANES = W * kWave / 16, PER = HD / LANES > 0 ? HD / LANES : 1;      // lanes of a row, entries of a lane
+  const int r = threadIdx.x / LANES, at = threadIdx.x % LANES * PER;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    l[rt] = rows_sum(l[rt]);
-    const float more = NT > 1 ? rows_sum(of_mid[rt]) : fmaf(-(B + 8.f), of_step[rt][0], rows_sum(of_mid[rt]));
+    const float all = rows_sum(l[rt]), more = NT > 1 ? rows_sum(of_mid[rt]) : fmaf(-(B + 8.f), of_step[rt][0], rows_sum(of_mid[rt]));
+    if (rt > 0) __syncthreads();
+    if (kq == 0) {
+      ms[wave][n16] = limit[rt] == -FLT_MAX ? -FLT_MAX : -less_m[rt][0];
+      ls[wave][n16] = all;
+    }
+    float top = -FLT_MAX, sum = 0.f, x[PER] = {};
 #pragma unroll
-    for (int d = 0; d < C; ++d) o[rt][d] += more;
-  }
-  if constexpr (!KEYS) {
+    for (int turn = 0; turn < W / 4; ++turn) {
+      if (turn > 0) __syncthreads();
+      if (wave / 4 == turn) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (first + 16 * rt + n16 >= span.rows) continue;
-      const float by = segs > 1 ? 1.f : l[rt] == 0.f ? 0.f : 1.f / l[rt];
-      float* left = segs > 1 ? scratch + ((static_cast<size_t>(row[rt]) * sh.nh + head[rt]) * sh.max_segs + part) * (HD + 2) : nullptr;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {      // lane kq has entries kq * HD / 4 on
-        float x[C];
-#pragma unroll
-        for (int d = 0; d < C; ++d) x[d] = o[rt][d][i] * by;
-        const int at = (4 * kq + i) * C;
-        if (segs > 1) {
-#pragma unroll
-          for (int d = 0; d < C; ++d) left[at + d] = x[d];
-        } else {
-          store_some(out + static_cast<size_t>(row[rt]) * sh.out_stride + head[rt] * HD + at, x);
-        }
+          for (int d = 0; d < C; ++d) os[wave % 4][n16][(4 * kq + i) * C + d] = o[rt][d][i] + more;
       }
-      if (segs > 1 && kq == 0) {
-        left[HD] = m[rt];
-        left[HD + 1] = l[rt];
+      __syncthreads();
+      if (turn == 0) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, ms[w][r]);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float by = __builtin_amdgcn_exp2f(ms[4 * turn + w][r] - top);
+        sum = fmaf(ls[4 * turn + w][r], by, sum);
+        if (at < HD) {
+#pragma unroll
+          for (int e = 0; e < PER; ++e) x[e] = fmaf(os[w][r][at + e], by, x[e]);
+        }
       }
     }
-  } else {
-    // Four waves at a time leave their sums in LDS; a row's lanes add them up, the waves in order.
-    __shared__ float os[4][16][HD + 4], ms[W][16], ls[W][16];
-    constexpr int LANES = W * kWave / 16, PER = HD / LANES > 0 ? HD / LANES : 1;      // lanes of a row, entries of a lane
-    const int r = threadIdx.x / LANES, at = threadIdx.x % LANES * PER;
+    const int f = first + 16 * rt + r;
+    if (f >= span.rows || at >= HD) continue;
+    const int of = quotient(f, sh.group), h = kvh * group + f - of * group;
+    const size_t to = span.row0 + of;
+    if (segs > 1) {
+      float* left = scratch + ((to * sh.nh + h) * sh.max_segs + part) * (HD + 2);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (rt > 0) __syncthreads();
-      if (kq == 0) {
-        ms[wave][n16] = m[rt];
-        ls[wave][n16] = l[rt];
+      for (int e = 0; e < PER; ++e) left[at + e] = x[e];
+      if (at == 0) {
+        left[HD] = top;
+        left[HD + 1] = sum;
       }
-      float top = -FLT_MAX, sum = 0.f, x[PER] = {};
+    } else {
+      const float by = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int turn = 0; turn < W / 4; ++turn) {
-        if (turn > 0) __syncthreads();
-        if (wave / 4 == turn) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int d = 0; d < C; ++d) os[wave % 4][n16][(4 * kq + i) * C + d] = o[rt][d][i];
-        }
-        __syncthreads();
-        if (turn == 0) {
-#pragma unroll
-          for (int w = 0; w < W; ++w) top = fmaxf(top, ms[w][r]);
-        }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float by = __builtin_amdgcn_exp2f((ms[4 * turn + w][r] - top) * sh.scale_log2);
-          sum = fmaf(ls[4 * turn + w][r], by, sum);
-          if (at < HD) {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) x[e] = fmaf(os[w][r][at + e], by, x[e]);
-          }
-        }
-      }
-      const int f = first + 16 * rt + r;
-      if (f >= span.rows || at >= HD) continue;
-      const int of = quotient(f, sh.group), h = kvh * group + f - of * group;
-      const size_t to = span.row0 + of;
-      if (segs > 1) {
-        float* left = scratch + ((to * sh.nh + h) * sh.max_segs + part) * (HD + 2);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) left[at + e] = x[e];
-        if (at == 0) {
-          left[HD] = top;
-          left[HD + 1] = sum;
-        }
-      } else {
-        const float by = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) x[e] *= by;
-        store_some(out + to * sh.out_stride + h * HD + at, x);
-      }
+      for (int e = 0; e < PER; ++e) x[e] *= by;
+      store_some(out + to * sh.out_stride + h * HD + at, x);
     }
   }
 }
@@ -548,7 +520,7 @@ __global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ 
   constexpr int PER = (HD + kWave - 1) / kWave;
   float sum = 0.f, x[PER] = {};
   for (int i = 0; i < segs; ++i, left += HD + 2) {
-    const float by = __builtin_amdgcn_exp2f((left[HD] - top) * sh.scale_log2);
+    const float by = __builtin_amdgcn_exp2f(left[HD] - top);
     sum = fmaf(left[HD + 1], by, sum);
 #pragma unroll
     for (int e = 0; e < PER; ++e)
@@ -562,25 +534,21 @@ __global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ 
 // ---- host side
 struct Plan {
   int rt, waves, segment, max_segs, tile_rows, tiles;
-  bool keys;
   long long floats;
 };
 
 constexpr long long kFill = 512;      // workgroups that fill the chip: two on each of 256 CUs
 constexpr int kWideChunks = 4;      // of a wave, at most, before contexts are cut
-constexpr int wide_waves(int hd) { return hd <= 64 ? 16 : 8; }      // (registers: 128 of a lane, and 256)
+constexpr int wide_waves(int hd) { return hd <= 64 ? 16 : hd == 128 ? 8 : 4; }      // (a lane's registers: 128, 256, and all)
 
 Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
   Plan p{};
   const int group = nh / nkv;
   max_run = std::min(max_run, T);
   const long long pairs = static_cast<long long>(max_run) * group;
-  const long long waves = static_cast<long long>(units) * nkv * ((pairs + 31) / 32);
-  p.keys = pairs <= 16 || waves < 2 * kFill;
-  p.rt = p.keys ? (pairs > 16 && hd <= 128 ? 2 : 1) : 2;
-  if (hd == 256) p.rt = 1;
-  p.waves = p.keys ? 4 : 1;
-  p.tile_rows = 16 * p.rt * (p.keys ? 1 : p.waves);
+  p.rt = pairs > 16 && hd <= 128 ? 2 : 1;
+  p.waves = 4;
+  p.tile_rows = 16 * p.rt;
   p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
   const long long groups = static_cast<long long>(units) * nkv * p.tiles;
   const long long seen = window > 0 && window + p.tile_rows < max_context ? window + p.tile_rows : max_context;
@@ -590,7 +558,7 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   if (parts < 1) parts = 1;
   // Few tokens: one workgroup of many waves instead of parts and a launch that joins them (32 heads over 4 of 64, one row of 529 tokens: 6.9
   // us, with parts 8.1).
-  if (p.keys && p.rt == 1 && parts > 1 && seen <= wide_waves(hd) * kChunk * kWideChunks) {
+  if (p.rt == 1 && wide_waves(hd) > 4 && parts > 1 && seen <= wide_waves(hd) * kChunk * kWideChunks) {
     parts = 1;
     p.waves = wide_waves(hd);
   }
@@ -620,10 +588,8 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
   s.q_stride = q_stride, s.out_stride = out_stride, s.table_stride = table_stride, s.nh = nh, s.pages = pages;
   s.max_segs = p.max_segs, s.tiles = p.tiles, s.tile_rows = p.tile_rows;
   s.nkv = divisor(nkv), s.group = divisor(nh / nkv), s.segs = divisor(p.max_segs), s.page_tiles = divisor(page / kTile4), s.segment = divisor(p.segment / kChunk);
-  s.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  s.scale_log2 = scale * 1.4426950408889634f;
   s.window = window, s.max_context = static_cast<int>(std::min<long long>(static_cast<long long>(table_stride) * page, max_context));
-  s.negate = scale < 0.f;
-  if (s.scale_log2 == 0.f) s.scale_log2 = 1e-30f;      // (0 times what has not seen a token yet would not be 0)
   const long long x = static_cast<long long>(nkv) * p.max_segs * p.tiles;
   KVCM_REQUIRE(x < (1ll << 30) && static_cast<long long>(rows.total) * (nh / nkv) < (1ll << 30) && units < 65536, "%s: %lld workgroups for each of %d sequences", what, x, units);
   KVCM_REQUIRE(p.max_segs == 1 || max_run < 65536, "%s: runs of %d rows cut into segments", what, max_run);
@@ -634,17 +600,14 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       const T* qt = static_cast<const T*>(q);
       T* ot = static_cast<T*>(out);
       const uint8_t* ct = static_cast<const uint8_t*>(cache);
-      const auto walk = [&](auto rt, auto waves, auto keys) {
-        attention4_kernel<T, HD, decltype(rt)::value, decltype(waves)::value, decltype(keys)::value>
-            <<<grid, decltype(waves)::value * kWave, 0, stream>>>(qt, ot, ct, tables, rows, s, scratch);
+      const auto walk = [&](auto rt, auto waves) {
+        attention4_kernel<T, HD, decltype(rt)::value, decltype(waves)::value><<<grid, decltype(waves)::value * kWave, 0, stream>>>(qt, ot, ct, tables, rows, s, scratch);
       };
       constexpr std::integral_constant<int, 1> one;
       constexpr std::integral_constant<int, 4> four;
-      constexpr std::integral_constant<int, HD == 256 ? 1 : 2> most;
-      if (!p.keys) walk(most, one, std::false_type());
-      else if (p.rt == 2) walk(most, four, std::true_type());
-      else if (p.waves == 4) walk(one, four, std::true_type());
-      else walk(one, std::integral_constant<int, wide_waves(HD)>(), std::true_type());
+      if (p.rt == 2) walk(std::integral_constant<int, HD == 256 ? 1 : 2>(), four);
+      else if (p.waves == 4) walk(one, four);
+      else walk(one, std::integral_constant<int, wide_waves(HD)>());
       if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), kWave, 0, stream>>>(scratch, ot, rows, s);
     };
     if (dtype == kBF16) go(bf16_t());
