@@ -31,6 +31,7 @@
 // waves make for one another in LDS, a quarter fewer instructions and a barrier every 64 tokens, 475 us.
 // Contexts are cut into segments that run as workgroups of their own while there are few; a second launch joins what they leave
 // in scratch (o, m, l in 32 bits, in the order of the segments).
+
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -63,6 +64,10 @@ __device__ __forceinline__ uint32_t codes(uint32_t word, int s, uint32_t mask) {
   if constexpr (B == 128) return (word >> (4 * s) & mask) | 0x43004300u;
   return ((s == 0 ? word << 3 : word >> (4 * s - 3)) & mask) | 0x41804180u;
 }
+
+// The low halves of two words side by side, and the high ones.
+__device__ __forceinline__ uint32_t pick_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t pick_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 // Numbers as sums of bfloat16 ones: one for rows of bfloat16, three for float (24 bits).
 template <class T> constexpr int kTerms = 1;
@@ -141,19 +146,11 @@ __device__ __forceinline__ Cut cut_of(const Span& p, const Shape& s, int block_f
   return Cut{first, hi > lo ? quotient((hi - 1) / kChunk, s.segment) - first + 1 : 1};
 }
 
-template <class T>
-__device__ __forceinline__ void load_eight(const T* p, float x[8]) {
-  if constexpr (sizeof(T) == 2) {
-    typedef uint16_t raw __attribute__((ext_vector_type(8), aligned(2)));
-    const raw r = *reinterpret_cast<const raw*>(p);
+__device__ __forceinline__ void load_eight(const float* p, float x[8]) {
+  typedef float raw __attribute__((ext_vector_type(4), aligned(4)));
+  const raw a = reinterpret_cast<const raw*>(p)[0], b = reinterpret_cast<const raw*>(p)[1];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = bf16_bits_to_float(r[i]);
-  } else {
-    typedef float raw __attribute__((ext_vector_type(4), aligned(4)));
-    const raw a = reinterpret_cast<const raw*>(p)[0], b = reinterpret_cast<const raw*>(p)[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = a[i], x[i + 4] = b[i];
-  }
+  for (int i = 0; i < 4; ++i) x[i] = a[i], x[i + 4] = b[i];
 }
 template <class T, int N>
 __device__ __forceinline__ void store_some(T* p, const float (&x)[N]) {
@@ -201,6 +198,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
   const int lo = max(first_of(span, sh, at_first), seg_first), hi = min(end_of(span, sh, at_last), seg_end);
   const int all_lo = first_of(span, sh, at_last), all_hi = end_of(span, sh, at_first);      // what every row sees
 
+  const u32x4 ones{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   int row_lo[RT], row_hi[RT];
   u32x4 qf[RT][NT][KS], q_sum[RT];
   f32x4 start[RT];
@@ -210,25 +208,32 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     const int at = quotient(f, sh.group), head = kvh * group + f - at * group;
     row_lo[rt] = max(first_of(span, sh, at), seg_first);
     row_hi[rt] = min(end_of(span, sh, at), seg_end);
-    float sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < KS; ++c) {
-      float x[8];
-      load_eight(q + static_cast<size_t>(span.row0 + at) * sh.q_stride + head * HD + kq * (HD / 4) + 8 * c, x);
+    for (int c = 0; c < KS; ++c) {      // codes come in the order 0 4 1 5 2 6 3 7
+      const T* from = q + static_cast<size_t>(span.row0 + at) * sh.q_stride + head * HD + kq * (HD / 4) + 8 * c;
+      if constexpr (NT == 1) {
+        typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(2)));
+        const raw x = *reinterpret_cast<const raw*>(from);
+        qf[rt][0][c] = u32x4{pick_low(x[0], x[2]), pick_high(x[0], x[2]), pick_low(x[1], x[3]), pick_high(x[1], x[3])};
+      } else {
+        float x[8];
+        load_eight(from, x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[i];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {      // codes come in the order 0 4 1 5 2 6 3 7
-          qf[rt][n][c][i] = pack(x[i], x[i + 4]);
-          if (n + 1 < NT) {
+          for (int i = 0; i < 4; ++i) {
+            qf[rt][n][c][i] = pack(x[i], x[i + 4]);
             x[i] -= bf16_bits_to_float(qf[rt][n][c][i] & 0xFFFFu);
             x[i + 4] -= bf16_bits_to_float(qf[rt][n][c][i] >> 16);
           }
-        }
+      }
     }
-    sum = rows_sum(sum);
+    f32x4 sums{0.f, 0.f, 0.f, 0.f};      // each of them the row's
+#pragma unroll
+    for (int n = NT - 1; n >= 0; --n)
+#pragma unroll
+      for (int c = 0; c < KS; ++c) sums = product(ones, qf[rt][n][c], sums);
+    const float sum = sums[0];
     const float less = -(B + 8.f) * sum;
     start[rt] = f32x4{less, less, less, less};      // (float rows)
     // against a pair (step, low), three times: what step and low are multiplied with (the first lane of a row; the others' is 0)
@@ -389,7 +394,6 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
             }
           }
     }
-    const u32x4 ones{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if constexpr (NT > 1) of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -445,8 +449,9 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     }
   }
 
-  // Four waves at a time leave their sums in LDS; a row's lanes add them up, the waves in order.
-  __shared__ float os[4][16][HD + 4], ms[W][16], ls[W][16];
+  // Up to four waves at a time leave their sums in LDS; a row's lanes add them up, the waves in order.
+  constexpr int AT_ONCE = W < 4 ? W : 4;
+  __shared__ float os[AT_ONCE][16][HD + 4], ms[W][16], ls[W][16];
   constexpr int LANES = W * kWave / 16, PER = HD / LANES > 0 ? HD / LANES : 1;      // lanes of a row, entries of a lane
   const int r = threadIdx.x / LANES, at = threadIdx.x % LANES * PER;
 #pragma unroll
@@ -459,13 +464,13 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     }
     float top = -FLT_MAX, sum = 0.f, x[PER] = {};
 #pragma unroll
-    for (int turn = 0; turn < W / 4; ++turn) {
+    for (int turn = 0; turn < W / AT_ONCE; ++turn) {
       if (turn > 0) __syncthreads();
-      if (wave / 4 == turn) {
+      if (wave / AT_ONCE == turn) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int d = 0; d < C; ++d) os[wave % 4][n16][(4 * kq + i) * C + d] = o[rt][d][i] + more;
+          for (int d = 0; d < C; ++d) os[wave % AT_ONCE][n16][(4 * kq + i) * C + d] = o[rt][d][i] + more;
       }
       __syncthreads();
       if (turn == 0) {
@@ -473,9 +478,9 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
         for (int w = 0; w < W; ++w) top = fmaxf(top, ms[w][r]);
       }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float by = __builtin_amdgcn_exp2f(ms[4 * turn + w][r] - top);
-        sum = fmaf(ls[4 * turn + w][r], by, sum);
+      for (int w = 0; w < AT_ONCE; ++w) {
+        const float by = __builtin_amdgcn_exp2f(ms[AT_ONCE * turn + w][r] - top);
+        sum = fmaf(ls[AT_ONCE * turn + w][r], by, sum);
         if (at < HD) {
 #pragma unroll
           for (int e = 0; e < PER; ++e) x[e] = fmaf(os[w][r][at + e], by, x[e]);
@@ -503,10 +508,15 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
   }
 }
 
-// Joins the segments of a row: one wave a (row, head).
+// Joins the segments of a row: a workgroup a (row, head).  Each thread weighs a segment; 256 / HD threads share an entry, a
+// segment in so many of them each, eight loads at a time under way.  (One wave that went through a row's 64 segments one after the other
+// took 50 us.)
+constexpr int kMostSegments = 1024;
 template <class T, int HD>
-__global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ scratch, T* __restrict__ out, Rows rows, Shape sh) {
-  const int head = blockIdx.x, group = sh.group.d, lane = threadIdx.x;
+__global__ void __launch_bounds__(256) join4_kernel(const float* __restrict__ scratch, T* __restrict__ out, Rows rows, Shape sh) {
+  constexpr int G = 256 / HD, AHEAD = 8;
+  __shared__ float weight[kMostSegments], sums[G][HD], of_wave[2][4];
+  const int head = blockIdx.x, group = sh.group.d, wave = threadIdx.x / kWave;
   const Span span = span_of(rows, sh, blockIdx.z);
   const int at = blockIdx.y;      // position in the span
   if (at * group >= span.rows) return;
@@ -515,20 +525,37 @@ __global__ void __launch_bounds__(kWave) join4_kernel(const float* __restrict__ 
   if (segs == 1) return;
   const size_t row = span.row0 + at;
   const float* left = scratch + (row * sh.nh + head) * sh.max_segs * (HD + 2);
-  float top = -FLT_MAX;
-  for (int i = 0; i < segs; ++i) top = fmaxf(top, left[i * (HD + 2) + HD]);
-  constexpr int PER = (HD + kWave - 1) / kWave;
-  float sum = 0.f, x[PER] = {};
-  for (int i = 0; i < segs; ++i, left += HD + 2) {
-    const float by = __builtin_amdgcn_exp2f(left[HD] - top);
-    sum = fmaf(left[HD + 1], by, sum);
-#pragma unroll
-    for (int e = 0; e < PER; ++e)
-      if (lane + e * kWave < HD) x[e] = fmaf(left[lane + e * kWave], by, x[e]);
+  float top = -FLT_MAX, sum = 0.f;
+  for (int i = threadIdx.x; i < segs; i += 256) top = fmaxf(top, left[i * (HD + 2) + HD]);
+  top = wave_max(top);
+  if (threadIdx.x % kWave == 0) of_wave[0][wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(of_wave[0][0], of_wave[0][1]), fmaxf(of_wave[0][2], of_wave[0][3]));
+  for (int i = threadIdx.x; i < segs; i += 256) {
+    const float by = __builtin_amdgcn_exp2f(left[i * (HD + 2) + HD] - top);
+    weight[i] = by;
+    sum = fmaf(left[i * (HD + 2) + HD + 1], by, sum);
   }
+  sum = wave_sum(sum);
+  if (threadIdx.x % kWave == 0) of_wave[1][wave] = sum;
+  __syncthreads();
+  const int e = threadIdx.x % HD, g = threadIdx.x / HD;
+  float x = 0.f;
+  for (int i = g; i < segs; i += AHEAD * G) {
+    float next[AHEAD];
 #pragma unroll
-  for (int e = 0; e < PER; ++e)
-    if (lane + e * kWave < HD) store_f(out + row * sh.out_stride + head * HD + lane + e * kWave, sum == 0.f ? 0.f : x[e] / sum);
+    for (int n = 0; n < AHEAD; ++n) next[n] = i + n * G < segs ? left[static_cast<size_t>(i + n * G) * (HD + 2) + e] : 0.f;
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) x = i + n * G < segs ? fmaf(next[n], weight[i + n * G], x) : x;
+  }
+  sums[g][e] = x;
+  __syncthreads();
+  if (g == 0) {
+#pragma unroll
+    for (int n = 1; n < G; ++n) x += sums[n][e];
+    sum = (of_wave[1][0] + of_wave[1][1]) + (of_wave[1][2] + of_wave[1][3]);
+    store_f(out + row * sh.out_stride + head * HD + e, sum == 0.f ? 0.f : x / sum);
+  }
 }
 
 // ---- host side
@@ -537,8 +564,9 @@ struct Plan {
   long long floats;
 };
 
-constexpr long long kFill = 512;      // workgroups that fill the chip: two on each of 256 CUs
-constexpr int kWideChunks = 4;      // of a wave, at most, before contexts are cut
+constexpr long long kFill = 768;      // workgroups that fill the chip: three on each of 256 CUs
+static_assert(kFill + 2 <= kMostSegments);
+constexpr int kWideChunks = 2;      // of a wave, at most, before contexts are cut
 constexpr int wide_waves(int hd) { return hd <= 64 ? 16 : hd == 128 ? 8 : 4; }      // (a lane's registers: 128, 256, and all)
 
 Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
@@ -552,18 +580,20 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
   const long long groups = static_cast<long long>(units) * nkv * p.tiles;
   const long long seen = window > 0 && window + p.tile_rows < max_context ? window + p.tile_rows : max_context;
-  long long parts = (kFill + groups - 1) / groups;
-  const int least = 8 * kChunk;      // tokens of a segment at least
-  if (parts > (seen + least - 1) / least) parts = (seen + least - 1) / least;
-  if (parts < 1) parts = 1;
-  // Few tokens: one workgroup of many waves instead of parts and a launch that joins them (32 heads over 4 of 64, one row of 529 tokens: 6.9
-  // us, with parts 8.1).
+  // Parts that fill the chip, but none shorter than a chunk of each wave, and no more than what joining them costs: a part more is some 0.07
+  // us of the second launch, a chunk less of every wave some 0.8 us of the first, the sum of both least at sqrt(12 seen / 128) parts
+  // (one row, 8 kv heads of 128: 8,192 tokens 64 parts 11.0 us, 32 parts 9.1; 2,048 tokens 16 parts 7.5 us, 8 parts 7.9).
+  constexpr int LEAST = 4 * kChunk;
+  long long parts = std::min((kFill + groups / 2) / groups, (seen + LEAST - 1) / LEAST);
+  while (parts > 1 && parts * parts * LEAST > 12 * seen) --parts;
+  parts = std::max(parts, 1ll);
+  // Few tokens: one workgroup of many waves instead, and no second launch (32 heads over 4 of 64, one row of 529 tokens: 7.0 us, with parts
+  // 6.8 and another launch for the host; 1,000 tokens 8.4 us and 6.9).
   if (p.rt == 1 && wide_waves(hd) > 4 && parts > 1 && seen <= wide_waves(hd) * kChunk * kWideChunks) {
     parts = 1;
     p.waves = wide_waves(hd);
   }
-  p.segment = static_cast<int>(((seen + parts - 1) / parts + least - 1) / least * least);
-  if (p.segment < least) p.segment = least;
+  p.segment = static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
   p.max_segs = parts == 1 ? 1 : static_cast<int>((max_context + p.segment - 1) / p.segment);
   if (parts > 1 && seen < max_context) p.max_segs = static_cast<int>((seen - 1) / p.segment + 2);
   p.floats = p.max_segs == 1 ? 0 : static_cast<long long>(T) * nh * p.max_segs * (hd + 2);
@@ -608,7 +638,7 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       if (p.rt == 2) walk(std::integral_constant<int, HD == 256 ? 1 : 2>(), four);
       else if (p.waves == 4) walk(one, four);
       else walk(one, std::integral_constant<int, wide_waves(HD)>());
-      if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), kWave, 0, stream>>>(scratch, ot, rows, s);
+      if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), 256, 0, stream>>>(scratch, ot, rows, s);
     };
     if (dtype == kBF16) go(bf16_t());
     else go(float());
