@@ -579,7 +579,7 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   p.tile_rows = 16 * p.rt;
   p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
   const long long groups = static_cast<long long>(units) * nkv * p.tiles;
-  const long long seen = window > 0 && window + p.tile_rows < max_context ? window + p.tile_rows : max_context;
+  const long long seen = window > 0 ? std::min<long long>(static_cast<long long>(window) + p.tile_rows, max_context) : max_context;
   // Parts that fill the chip, but none shorter than a chunk of each wave, and no more than what joining them costs: a part more is some 0.07
   // us of the second launch, a chunk less of every wave some 0.8 us of the first, the sum of both least at sqrt(12 seen / 128) parts
   // (one row, 8 kv heads of 128: 8,192 tokens 64 parts 11.0 us, 32 parts 9.1; 2,048 tokens 16 parts 7.5 us, 8 parts 7.9).
@@ -594,7 +594,7 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
     p.waves = wide_waves(hd);
   }
   p.segment = static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
-  p.max_segs = parts == 1 ? 1 : static_cast<int>((max_context + p.segment - 1) / p.segment);
+  p.max_segs = parts == 1 ? 1 : static_cast<int>((static_cast<long long>(max_context) + p.segment - 1) / p.segment);
   if (parts > 1 && seen < max_context) p.max_segs = static_cast<int>((seen - 1) / p.segment + 2);
   p.floats = p.max_segs == 1 ? 0 : static_cast<long long>(T) * nh * p.max_segs * (hd + 2);
   return p;

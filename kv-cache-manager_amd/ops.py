@@ -1338,7 +1338,7 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
     """``attention`` over a 4-bit cache for rows of different sequences (bfloat16 or float32): out[r, h] = softmax(scale * q[r, h] . K) V
     over the tokens 0 .. ctx_lens[r] - 1 of sequence row_seq[r] (``window`` > 0: the last ``window`` of them).  A row that sees nothing (a
     context of 0, a sequence without a table) gives zeros, and so would one whose pages all lie outside the cache: a table's entry that is
-    no page hides its tokens.  ``max_context`` bounds every row's context length and decides how contexts are cut into parts that run side
+    no page hides its tokens.  ``max_context`` bounds every row's context length (what lies beyond it is not looked at) and decides how contexts are cut into parts that run side
     by side, which needs ``scratch`` (attention_decode4_scratch floats; allocated here when not given)."""
     T = q.shape[0] if rows is None else rows
     q_at, out_at, cache_at, tables_at, seq_at, lens_at, scratch_at = _one_gpu(q, out, cache, tables, row_seq, ctx_lens, scratch)
@@ -1351,8 +1351,8 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
     _i32(tables, "tables")
     if not held >= table_stride > 0:
         raise ValueError("tables must hold rows of table_stride pages")
-    if window < 0 or max_context < 0:
-        raise ValueError("window and max_context must not be negative")
+    if not (0 <= window < 2 ** 31 and 0 <= max_context < 2 ** 31):
+        raise ValueError("window and max_context must be from 0 on and fit 32 bits")
     need, floats = attention_decode4_scratch(T, nh, nkv, hd, max_context, window), 0
     if need or scratch is not None:
         scratch, floats = _scratch4("attention_decode4", need, scratch, q.device)
@@ -1378,14 +1378,14 @@ def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
     dtype, cols = q.dtype, nh * hd
     q_stride, out_stride = _long_rows(q, "q", T, cols, dtype), _long_rows(out, "out", T, cols, dtype)
-    if table_stride <= 0 or num_seqs < 0 or max_run < 0 or window < 0:
-        raise ValueError("table_stride must be positive, num_seqs, max_run and window not negative")
+    if not (table_stride > 0 and num_seqs >= 0 and 0 <= max_run < 2 ** 31 and 0 <= window < 2 ** 31):
+        raise ValueError("table_stride must be positive, num_seqs, max_run and window from 0 on and fit 32 bits")
     _i32(run_start, "run_start", num_seqs + 1)
     _i32(seq_start, "seq_start", num_seqs)
     _i32(tables, "tables", num_seqs * table_stride)
     max_context = table_stride * page if max_context is None else max_context
-    if max_context < 0:
-        raise ValueError("max_context must not be negative")
+    if not 0 <= max_context < 2 ** 31:
+        raise ValueError("max_context must be from 0 on and fit 32 bits")
     need, floats = attention_prefill4_scratch(T, nh, nkv, hd, max_context, max_run, num_seqs, window), 0
     if need or scratch is not None:
         scratch, floats = _scratch4("attention_prefill4", need, scratch, q.device)

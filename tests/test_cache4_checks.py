@@ -144,3 +144,38 @@ def test_the_shape_of_a_cache():
     for bad in ((0, 4, 64, 16), (7, 4, 48, 16), (7, 4, 64, 24), (7, 0, 64, 16)):
         with pytest.raises(ValueError, match="4-bit cache"):
             ops.cache4_shape(*bad)
+
+
+def test_numbers_that_do_not_fit_are_refused():
+    for call in (decode, prefill):
+        for bad in (dict(window=2 ** 31), dict(max_context=2 ** 32 + 5)):
+            with pytest.raises(ValueError, match="fit 32 bits"):
+                call(**bad)
+    with pytest.raises(ValueError, match="fit 32 bits"):
+        prefill(max_run=2 ** 31)
+    said, p, lib = lambda: ops.lib().kvcm_hip_last_error().decode(), 4096, ops.lib()
+    assert lib.kvcm_rope_cache4(p, 1, 512, 0, 0, p, p, 0, 2 ** 28, 4, 2, 64, 9, 32, 0) == -1 and "too many" in said()
+    assert lib.kvcm_cache4_rows(p, p, p, 512, p, 512, 1, 2 ** 28, 8, 64, 9, 32, 0) == -1 and "too many" in said()
+    assert lib.kvcm_attention_decode4(p, 1, 256, p, 256, p, p, 4, 2, p, p, 70000, 4, 2, 64, 9, 32, 0.1, 0, 100, 0, 0, 0) == -1 and "70000" in said()
+    assert lib.kvcm_attention_prefill4(p, 1, 256, p, 256, p, p, 4, p, p, 2, 2 ** 30, 2 ** 30, 4, 2, 64, 9, 32, 0.1, 0, 100, 0, 0, 0) == -1 and "workgroups" in said()
+    assert lib.kvcm_attention_decode4_scratch(1, 4, 2, 64, 2 ** 31 - 1, 2 ** 31 - 1) >= 0
+
+
+def test_operands_elsewhere_are_refused(monkeypatch):
+    monkeypatch.undo()
+    for call in (store, read, decode, prefill):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+
+
+@pytest.mark.parametrize("nh, nkv, hd", ((32, 4, 64), (32, 8, 128), (16, 2, 256), (3, 1, 32)))
+def test_scratch_of_any_size_is_bounded(nh, nkv, hd):
+    """Parts fill the chip, whatever the contexts: scratch stays a small part of what the cache takes, and grows with nothing but the rows."""
+    for rows in (1, 3, 17, 64, 500, 5000):
+        for ctx in (0, 1, 100, 513, 4096, 33000, 2 ** 20, 2 ** 30):
+            for window in (0, 1, 4096):
+                floats = ops.attention_decode4_scratch(rows, nh, nkv, hd, ctx, window)
+                assert 0 <= floats <= (1024 // nkv + 3 * rows) * nh * (hd + 2), (rows, ctx, window)
+                assert ctx > 256 or floats == 0
+                runs = ops.attention_prefill4_scratch(rows, nh, nkv, hd, ctx, rows, 1, window)
+                assert 0 <= runs <= rows * nh * 1024 * (hd + 2)

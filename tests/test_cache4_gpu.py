@@ -331,3 +331,231 @@ def test_pages_that_are_none_hide_their_tokens(ops):
     runs = torch.empty(2, nh * hd, dtype=BF, device=DEV)
     ops.attention_prefill4(q, runs, s.cache, tables.view(-1), s.stride, ints([0, 1, 2]), ints([63, 63]), 2, 1, nh, nkv, hd, 0.125)
     near(runs, want, tol)
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+def test_other_places_signs_and_ranges(ops, dtype):
+    """Rows from any element on (2 or 4 bytes of alignment), a negative scale, keys and values far from 0 and far apart in size."""
+    nh, nkv, hd, page = 6, 2, 64, 32
+    gen = torch.Generator().manual_seed(11)
+    lengths = (77, 200, 31)
+    s = Sequences(ops, nh, nkv, hd, page, lengths, gen, dtype)
+    x = torch.randn(sum(lengths), 3 * nkv * hd, generator=gen) * torch.exp(3 * torch.randn(sum(lengths), 1, generator=gen)) + 5 * torch.randn(3 * nkv * hd, generator=gen)
+    wide = torch.zeros(sum(lengths), 3 * nkv * hd + 9, dtype=dtype, device=DEV)
+    wide[:, 3:-6] = x.to(dtype).to(DEV)
+    ops.rope_cache4(wide[:, 3:-6], nkv, nkv, hd, s.cache, torch.cat(s.slots).to(torch.int32))
+    s.held = plain.parts(s.cache, nkv, hd)
+    q = queries(3, nh * hd, dtype, gen, extra=5)
+    out = torch.full((3, nh * hd + 7), 9.0, dtype=dtype, device=DEV)
+    for scale in (0.05, -0.05):
+        want, tol = s.expect(q[:, 1:nh * hd + 1], range(3), [(0, n) for n in lengths], scale)
+        ops.attention_decode4(q[:, 1:], out[:, 5:], s.cache, s.dev_tables, s.stride, ints(range(3)), ints(lengths), nh, nkv, hd, scale, max(lengths))
+        near(out[:, 5:nh * hd + 5], want, tol)
+        ops.attention_prefill4(q[:, 1:], out[:, 1:], s.cache, s.dev_tables, s.stride, ints(range(4)), ints(n - 1 for n in lengths), 3, 1, nh, nkv, hd, scale)
+        near(out[:, 1:nh * hd + 1], want, tol)
+        assert bool((out[:, nh * hd + 5:] == 9).all()) and bool((out[:, 0] == 9).all())
+
+
+def test_scores_that_rise_and_fall_along_a_context(ops):
+    """m follows late (scores up to 2^6 above it are taken as they are): steps of every size up and down, in every wave's tokens."""
+    nh, nkv, hd, page, n = 2, 1, 32, 16, 700
+    gen = torch.Generator().manual_seed(12)
+    for dtype in (BF, F32):
+        s = Sequences(ops, nh, nkv, hd, page, (n,), gen, dtype)
+        along = torch.cumsum(torch.randn(n, generator=gen), 0) * torch.linspace(0.1, 3, n)
+        x = torch.randn(n, 3 * hd, generator=gen)
+        x[:, hd:2 * hd] += along.view(-1, 1)
+        ops.rope_cache4(x.to(dtype).to(DEV), 1, 1, hd, s.cache, s.slots[0].to(torch.int32))
+        s.held = plain.parts(s.cache, nkv, hd)
+        q = queries(n, nh * hd, dtype, gen) + 0.3
+        out = torch.empty(n, nh * hd, dtype=dtype, device=DEV)
+        ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints([0, n]), ints([0]), 1, n, nh, nkv, hd, hd ** -0.5)
+        want, tol = s.expect(q, [0] * n, [(0, p + 1) for p in range(n)], hd ** -0.5)
+        near(out, want, tol)
+        one = torch.empty(n, nh * hd, dtype=dtype, device=DEV)
+        ops.attention_decode4(q, one, s.cache, s.dev_tables, s.stride, ints([0] * n), ints(range(1, n + 1)), nh, nkv, hd, hd ** -0.5, n)
+        near(one, want, tol)
+
+
+def test_a_cache_of_more_than_4_gib(ops):
+    nh, nkv, hd, page = 4, 2, 256, 16
+    pages = (1 << 32) // (nkv * 16 * (hd + 8)) + 40
+    gen = torch.Generator().manual_seed(13)
+    cache = torch.empty(ops.cache4_shape(pages, nkv, hd, page), dtype=torch.uint8, device=DEV)
+    n = 50
+    mine = [pages - 1, 3, pages - 7, pages - 20]
+    slots = torch.tensor([mine[t // page] * page + t % page for t in range(n)], dtype=torch.int32, device=DEV)
+    x = torch.randn(n, 3 * nkv * hd, generator=gen).to(BF).to(DEV)
+    ops.rope_cache4(x, nkv, nkv, hd, cache, slots)
+    k, v = (torch.empty(n, nkv * hd, dtype=F32, device=DEV) for _ in range(2))
+    ops.cache4_rows(cache, slots, k, v)
+    small, there = torch.zeros(ops.cache4_shape(4, nkv, hd, page), dtype=torch.uint8, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV)
+    ops.rope_cache4(x, nkv, nkv, hd, small, there)
+    k2, v2 = (torch.empty_like(k) for _ in range(2))
+    ops.cache4_rows(small, there, k2, v2)
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+    q = queries(1, nh * hd, BF, gen)
+    one, two = torch.empty_like(q), torch.empty_like(q)
+    ops.attention_decode4(q, one, cache, ints(mine), 4, ints([0]), ints([n]), nh, nkv, hd, 0.06, n)
+    ops.attention_decode4(q, two, small, ints(range(4)), 4, ints([0]), ints([n]), nh, nkv, hd, 0.06, n)
+    assert torch.equal(one, two)
+
+
+class Served:
+    """A few sequences on their way through a model's attention: a prompt's portion or a token of each at a time, written and attended over."""
+
+    def __init__(self, ops, nh, nkv, hd, page, room, seqs, dtype, seed):
+        self.gen = torch.Generator().manual_seed(seed)
+        self.size = (nh, nkv, hd)
+        self.ops, self.page, self.dtype, self.stride = ops, page, dtype, -(-room // page)
+        pages = seqs * self.stride + 1
+        self.tables = torch.randperm(pages, generator=self.gen)[:seqs * self.stride].to(torch.int32).to(DEV).view(seqs, -1)
+        self.cache = garbage(ops, pages, nkv, hd, page, self.gen)
+        self.room, self.lens = room, [0] * seqs
+        self.buffers = {}
+
+    def inputs(self, runs):
+        """A step's rows, runs[i] of sequence i, in buffers that stay where they are from one step of the same runs to the next."""
+        nh, nkv, hd = self.size
+        T = sum(runs)
+        seq = [i for i, r in enumerate(runs) for _ in range(r)]
+        pos = [self.lens[i] + j for i, r in enumerate(runs) for j in range(r)]
+        table = self.tables.cpu()
+        angle = torch.tensor(pos).view(-1, 1) * 10000.0 ** (-torch.arange(hd // 2) * 2 / hd)
+        new = dict(qkv=torch.randn(T, (nh + 2 * nkv) * hd, generator=self.gen).to(self.dtype), slots=torch.tensor([int(table[s, p // self.page]) * self.page + p % self.page for s, p in zip(seq, pos)]),
+                   cos_sin=torch.stack([angle.cos(), angle.sin()], -1), seq=torch.tensor(seq), ctx=torch.tensor(pos) + 1,
+                   run_start=torch.tensor([0] + list(np.cumsum(runs))), seq_start=torch.tensor(self.lens))
+        for i, r in enumerate(runs):
+            self.lens[i] += r
+        held = self.buffers.setdefault(tuple(runs), {k: torch.empty(v.shape, dtype=v.dtype if v.is_floating_point() else torch.int32, device=DEV) for k, v in new.items()}
+                                       | dict(q=torch.empty(T, nh * hd, dtype=self.dtype, device=DEV), out=torch.empty(T, nh * hd, dtype=self.dtype, device=DEV),
+                                              k=torch.empty(T, nkv * hd, dtype=self.dtype, device=DEV), v=torch.empty(T, nkv * hd, dtype=self.dtype, device=DEV)))
+        for k, v in new.items():
+            held[k].copy_(v)
+        return held
+
+    def step(self, b, runs, scratch=None):
+        nh, nkv, hd = self.size
+        self.ops.rope_cache4(b["qkv"], nh, nkv, hd, self.cache, b["slots"], cos_sin=b["cos_sin"], q_out=b["q"])
+        if max(runs) == 1:
+            self.ops.attention_decode4(b["q"], b["out"], self.cache, self.tables.view(-1), self.stride, b["seq"], b["ctx"], nh, nkv, hd, hd ** -0.5, self.room, scratch=scratch)
+        else:
+            self.ops.attention_prefill4(b["q"], b["out"], self.cache, self.tables.view(-1), self.stride, b["run_start"], b["seq_start"], len(runs), max(runs), nh, nkv, hd,
+                                        hd ** -0.5, max_context=self.room, scratch=scratch)
+        self.ops.cache4_rows(self.cache, b["slots"], b["k"], b["v"])
+
+    def check(self, b):
+        """The outputs against 64 bits over what the cache holds now; what was read back against the same."""
+        nh, nkv, hd = self.size
+        held = plain.parts(self.cache, nkv, hd)
+        t = torch.arange(self.room, device=DEV)
+        slots = [(self.tables[i].long()[t // self.page] * self.page + t % self.page) for i in range(len(self.lens))]
+        rows = b["q"].shape[0]
+        some = sorted(set(range(0, rows, 5)) | {rows - 1})
+        want, tol = plain.attend(b["q"][some].double().view(-1, nh, hd), held, [slots[int(b["seq"][r])] for r in some], [(0, int(b["ctx"][r])) for r in some], nh, nkv, hd ** -0.5, self.dtype)
+        near(b["out"][some], want, tol)
+        at = b["slots"].long()
+        kc, ks, kl, vc, vs, vl = held
+        assert torch.equal(b["k"], (kl + ks * kc)[at].flatten(1).to(self.dtype)) and torch.equal(b["v"], (vl + vs * vc)[at].flatten(1).to(self.dtype))
+        # and the cache holds what was written: the rotated keys' range, an entry off by a step at most
+        x = b["qkv"].double().view(rows, -1, hd)[:, nh + nkv:]
+        assert bool(((b["v"].double().view(rows, nkv, hd) - x).abs() <= vs[at] * 0.6 + 2.0 ** -8 * x.abs().amax(-1, keepdim=True)).all())
+
+
+@pytest.mark.parametrize("nh, nkv, hd, page, dtype", ((8, 2, 64, 16, BF), (4, 1, 128, 48, BF), (4, 4, 32, 32, F32)))
+def test_steps_as_they_are_served(ops, nh, nkv, hd, page, dtype):
+    """Prompts in portions, then tokens: every step's rows attend over what the steps before have left in the pages."""
+    w = Served(ops, nh, nkv, hd, page, 400, 3, dtype, 21)
+    for runs in ((40, 1, 130), (1, 200, 3), (7, 2, 1), (1, 1, 1), (1, 1, 1), (20, 1, 1)):
+        b = w.inputs(runs)
+        w.step(b, runs)
+        w.check(b)
+
+
+@pytest.mark.parametrize("how", ("graph", "program"))
+@pytest.mark.parametrize("runs, before, room", (((1, 1, 1), (290, 3, 90), 700), ((1,), (3000,), 4000), ((9, 1, 64), (30, 300, 0), 700)))
+def test_steps_captured_and_replayed(ops, how, runs, before, room):
+    """A captured (or recorded) step replayed with other rows, other lengths and other pages' contents, eager steps in between: every replay
+    gives what the eager step gives, bit for bit."""
+    nh, nkv, hd, page = 8, 2, 64, 16
+    w = Served(ops, nh, nkv, hd, page, room, len(runs), BF, 22)
+    w.lens = list(before)
+    w.cache.zero_()
+    T = sum(runs)
+    need = (ops.attention_decode4_scratch(T, nh, nkv, hd, room) if max(runs) == 1
+            else ops.attention_prefill4_scratch(T, nh, nkv, hd, room, max(runs), len(runs)))
+    scratch = torch.empty(max(need, 1), dtype=F32, device=DEV)
+    b = w.inputs(runs)
+    w.step(b, runs, scratch)
+    torch.cuda.synchronize()
+    if how == "graph":
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            w.step(b, runs, scratch)
+        again = graph.replay
+    else:
+        program = ops.StepProgram()
+        with ops.recording(program):
+            w.step(b, runs, scratch)
+        assert len(program) == 3
+        again = program.run
+    for _ in range(4):
+        b = w.inputs(runs)
+        for x in ("q", "out", "k", "v"):
+            b[x].zero_()
+        again()
+        torch.cuda.synchronize()
+        w.check(b)
+        got = {x: b[x].clone() for x in ("q", "out", "k", "v")}
+        w.step(b, runs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(b[x], got[x]) for x in got)
+
+
+def test_two_graphs_with_one_scratch(ops):
+    """Two captured steps of different sizes share a scratch buffer; replayed in turn on one stream, each is right every time."""
+    nh, nkv, hd, page = 8, 1, 64, 16
+    need = max(ops.attention_decode4_scratch(r, nh, nkv, hd, 5000) for r in (1, 2))
+    assert need > 0
+    scratch, stream, work = torch.empty(need, dtype=F32, device=DEV), torch.cuda.Stream(), []
+    for r, before in ((1, (4000,)), (2, (3000, 1200))):
+        w = Served(ops, nh, nkv, hd, page, 5000, r, BF, 30 + r)
+        w.lens, runs = list(before), (1,) * r
+        w.cache.zero_()
+        b = w.inputs(runs)
+        w.step(b, runs, scratch)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            w.step(b, runs, scratch)
+        work.append((w, runs, graph))
+    for _ in range(3):
+        held = [w.inputs(runs) for w, runs, _ in work]
+        scratch.fill_(float("nan"))
+        for _, _, graph in work + work[:1]:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (w, _, _), b in zip(work, held):
+            w.check(b)
+
+
+def test_work_goes_to_the_current_stream(ops):
+    """On a side stream behind a long copy chain: what is read there is what the stream's earlier work has written."""
+    w = Served(ops, 8, 2, 64, 16, 300, 2, BF, 41)
+    w.lens = [100, 250]
+    w.cache.zero_()
+    runs = (1, 1)
+    b = w.inputs(runs)
+    rows = b["qkv"].clone()
+    torch.cuda.synchronize()
+    stream, big = torch.cuda.Stream(), torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    with torch.cuda.stream(stream):
+        b["qkv"].zero_()
+        for _ in range(4):
+            big.copy_(big.flip(0))
+        b["qkv"].copy_(rows)
+        w.step(b, runs)
+    stream.synchronize()
+    w.check(b)
