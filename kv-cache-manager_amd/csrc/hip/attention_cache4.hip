@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
 // Joins the segments of a row: a workgroup a (row, head).  Each thread weighs a segment; 256 / HD threads share an entry, a
 // segment in so many of them each, eight loads at a time under way.  (One wave that went through a row's 64 segments one after the other
 // took 50 us.)
-constexpr int kMostSegments = 1024;
+constexpr int kMostSegments = 1600;
 template <class T, int HD>
 __global__ void __launch_bounds__(256) join4_kernel(const float* __restrict__ scratch, T* __restrict__ out, Rows rows, Shape sh) {
   constexpr int G = 256 / HD, AHEAD = 8;
@@ -565,9 +565,16 @@ struct Plan {
 };
 
 constexpr long long kFill = 768;      // workgroups that fill the chip: three on each of 256 CUs
-static_assert(kFill + 2 <= kMostSegments);
-constexpr int kWideChunks = 2;      // of a wave, at most, before contexts are cut
-constexpr int wide_waves(int hd) { return hd <= 64 ? 16 : hd == 128 ? 8 : 4; }      // (a lane's registers: 128, 256, and all)
+static_assert(2 * kFill + 2 <= kMostSegments);
+
+// What a call with its contexts cut into `parts` takes, roughly: a round of 128 tokens (a chunk of each wave) is 0.8 us where the chip is
+// nearly empty and 2.5 where it is full; joining is a launch, the parts that a row's workgroup goes through, the workgroups, and the bytes.
+// One row, 8 kv heads of 128: 8,192 tokens take 11.0 us in 64 parts and 9.1 in 32; 2,048 tokens 7.5 us in 16 and 7.9 in 8.
+double expected_us(long long parts, long long groups, long long rounds, long long T, int nh, int hd) {
+  const long long passes = (groups * parts + kFill - 1) / kFill;
+  const double load = static_cast<double>(groups * parts) / (passes * kFill), walk = passes * ((rounds + parts - 1) / parts) * (0.8 + 1.7 * load);
+  return parts == 1 ? walk : walk + 2.5 + 0.07 * parts + static_cast<double>(T) * nh * (0.0008 + parts * (hd + 2) * 8 / 3e6);
+}
 
 Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
   Plan p{};
@@ -580,18 +587,22 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
   const long long groups = static_cast<long long>(units) * nkv * p.tiles;
   const long long seen = window > 0 ? std::min<long long>(static_cast<long long>(window) + p.tile_rows, max_context) : max_context;
-  // Parts that fill the chip, but none shorter than a chunk of each wave, and no more than what joining them costs: a part more is some 0.07
-  // us of the second launch, a chunk less of every wave some 0.8 us of the first, the sum of both least at sqrt(12 seen / 128) parts
-  // (one row, 8 kv heads of 128: 8,192 tokens 64 parts 11.0 us, 32 parts 9.1; 2,048 tokens 16 parts 7.5 us, 8 parts 7.9).
-  constexpr int LEAST = 4 * kChunk;
-  long long parts = std::min((kFill + groups / 2) / groups, (seen + LEAST - 1) / LEAST);
-  while (parts > 1 && parts * parts * LEAST > 12 * seen) --parts;
-  parts = std::max(parts, 1ll);
-  // Few tokens: one workgroup of many waves instead, and no second launch (32 heads over 4 of 64, one row of 529 tokens: 7.0 us, with parts
-  // 6.8 and another launch for the host; 1,000 tokens 8.4 us and 6.9).
-  if (p.rt == 1 && wide_waves(hd) > 4 && parts > 1 && seen <= wide_waves(hd) * kChunk * kWideChunks) {
+  // How many parts contexts are cut into: what the model makes least, among 1 2 3 4 6 8 12 16 .. and what fills the chip once.
+  constexpr int LEAST = 4 * kChunk;      // a chunk of each wave
+  const long long rounds = (seen + LEAST - 1) / LEAST, most = std::min(2 * kFill / groups, rounds);
+  long long parts = 1;
+  double least = expected_us(1, groups, rounds, T, nh, hd);
+  const auto consider = [&](long long n) {
+    const double us = n > 1 && n <= most ? expected_us(n, groups, rounds, T, nh, hd) : least;
+    if (us < least) least = us, parts = n;
+  };
+  for (long long n = 2; n <= most; n += n & (n - 1) ? n / 3 : n / 2) consider(n);
+  consider(kFill / groups);
+  // Few workgroups and up to 1,024 tokens: eight waves instead of four, and no parts (32 heads over 4 of 64, one row: 529 tokens 5.7 us, with
+  // four waves 6.2; 1,000 tokens 7.4 us, in parts 6.9 and a second launch for the host).
+  if (p.rt == 1 && hd <= 128 && groups <= 256 && rounds > 2 && seen <= 1024) {
     parts = 1;
-    p.waves = wide_waves(hd);
+    p.waves = 8;
   }
   p.segment = static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
   p.max_segs = parts == 1 ? 1 : static_cast<int>((static_cast<long long>(max_context) + p.segment - 1) / p.segment);
@@ -637,7 +648,7 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       constexpr std::integral_constant<int, 4> four;
       if (p.rt == 2) walk(std::integral_constant<int, HD == 256 ? 1 : 2>(), four);
       else if (p.waves == 4) walk(one, four);
-      else walk(one, std::integral_constant<int, wide_waves(HD)>());
+      else walk(one, std::integral_constant<int, HD == 256 ? 4 : 8>());
       if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), 256, 0, stream>>>(scratch, ot, rows, s);
     };
     if (dtype == kBF16) go(bf16_t());

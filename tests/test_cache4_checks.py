@@ -175,7 +175,7 @@ def test_scratch_of_any_size_is_bounded(nh, nkv, hd):
         for ctx in (0, 1, 100, 513, 4096, 33000, 2 ** 20, 2 ** 30):
             for window in (0, 1, 4096):
                 floats = ops.attention_decode4_scratch(rows, nh, nkv, hd, ctx, window)
-                assert 0 <= floats <= (1024 // nkv + 3 * rows) * nh * (hd + 2), (rows, ctx, window)
+                assert 0 <= floats <= (1536 // nkv + 3 * rows) * nh * (hd + 2), (rows, ctx, window)
                 assert ctx > 256 or floats == 0
                 runs = ops.attention_prefill4_scratch(rows, nh, nkv, hd, ctx, rows, 1, window)
-                assert 0 <= runs <= rows * nh * 1024 * (hd + 2)
+                assert 0 <= runs <= rows * nh * (1536 // nkv + 2) * (hd + 2)
