@@ -604,6 +604,13 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
     parts = 1;
     p.waves = 8;
   }
+  // Many workgroups of few rounds: two waves, whose beginning and end (half of a short walk) are half as many (32 heads over 8 of 128: 128 rows
+  // of 300 tokens 12.0 us, with four waves 14.8; 256 of 1,000 59.9 and 54.9.  Over 4 of 64: eight prompts of 128 tokens 7.9 us and 11.0, one of
+  // 1,024 21.1 and 17.9).
+  if (parts == 1 && groups >= 1024 && (p.rt == 1 ? 3 : 2) * seen <= groups) p.waves = 2;
+  // Of 256 entries a CU holds four waves: two workgroups where there are enough (16 heads over 2: 200 rows of 300 tokens 11.7 us, with four
+  // waves 16.4; a prompt of 2,048 91 and 108).
+  if (parts == 1 && groups > 256 && hd == 256) p.waves = 2;
   p.segment = static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
   p.max_segs = parts == 1 ? 1 : static_cast<int>((static_cast<long long>(max_context) + p.segment - 1) / p.segment);
   if (parts > 1 && seen < max_context) p.max_segs = static_cast<int>((seen - 1) / p.segment + 2);
@@ -646,7 +653,11 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       };
       constexpr std::integral_constant<int, 1> one;
       constexpr std::integral_constant<int, 4> four;
-      if (p.rt == 2) walk(std::integral_constant<int, HD == 256 ? 1 : 2>(), four);
+      constexpr std::integral_constant<int, 2> two;
+      constexpr std::integral_constant<int, HD == 256 ? 1 : 2> most;
+      if (p.rt == 2 && p.waves == 2) walk(most, two);
+      else if (p.rt == 2) walk(most, four);
+      else if (p.waves == 2) walk(one, two);
       else if (p.waves == 4) walk(one, four);
       else walk(one, std::integral_constant<int, HD == 256 ? 4 : 8>());
       if (p.max_segs > 1) join4_kernel<T, HD><<<dim3(nh, max_run, units), 256, 0, stream>>>(scratch, ot, rows, s);

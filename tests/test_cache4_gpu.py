@@ -559,3 +559,32 @@ def test_work_goes_to_the_current_stream(ops):
         w.step(b, runs)
     stream.synchronize()
     w.check(b)
+
+
+@pytest.mark.parametrize("nh, nkv, hd, rows, dtype", ((4, 4, 64, 300, BF), (8, 4, 32, 300, F32), (12, 12, 128, 90, BF), (2, 2, 256, 140, BF), (2, 2, 256, 140, F32)))
+def test_many_rows_of_short_contexts(ops, nh, nkv, hd, rows, dtype):
+    gen = torch.Generator().manual_seed(rows + hd)
+    lengths = torch.randint(0, 75, (rows,), generator=gen).tolist()
+    s = Sequences(ops, nh, nkv, hd, 16, lengths, gen, dtype)
+    q, out = queries(rows, nh * hd, dtype, gen), torch.full((rows, nh * hd), 9.0, dtype=dtype, device=DEV)
+    for window in (0, 33):
+        ops.attention_decode4(q, out, s.cache, s.dev_tables, s.stride, ints(range(rows)), ints(lengths), nh, nkv, hd, hd ** -0.5, 75, window=window)
+        some = list(range(0, rows, 3))
+        want, tol = s.expect(q[some], some, [(max(0, lengths[r] - window) if window else 0, lengths[r]) for r in some], hd ** -0.5)
+        near(out[some], want, tol)
+
+
+@pytest.mark.parametrize("nh, nkv, hd, seqs, dtype", ((32, 4, 64, 40, BF), (8, 8, 128, 60, BF), (16, 2, 32, 70, F32), (8, 1, 256, 40, BF)))
+def test_many_short_prompts(ops, nh, nkv, hd, seqs, dtype):
+    gen = torch.Generator().manual_seed(seqs + hd)
+    runs = torch.randint(1, 70, (seqs,), generator=gen).tolist()
+    starts = [0 if i % 3 else i for i in range(seqs)]
+    s = Sequences(ops, nh, nkv, hd, 16, [r + p for r, p in zip(runs, starts)], gen, dtype)
+    first = np.concatenate([[0], np.cumsum(runs)])
+    T = int(first[-1])
+    q, out = queries(T, nh * hd, dtype, gen), torch.full((T, nh * hd), 9.0, dtype=dtype, device=DEV)
+    ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints(first), ints(starts), seqs, max(runs), nh, nkv, hd, hd ** -0.5, max_context=140)
+    seq, pos = [i for i, r in enumerate(runs) for _ in range(r)], [p + j for r, p in zip(runs, starts) for j in range(r)]
+    some = list(range(0, T, 31)) + [T - 1]
+    want, tol = s.expect(q[some], [seq[i] for i in some], [(0, pos[i] + 1) for i in some], hd ** -0.5)
+    near(out[some], want, tol)
