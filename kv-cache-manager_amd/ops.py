@@ -1378,8 +1378,8 @@ def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
     dtype, cols = q.dtype, nh * hd
     q_stride, out_stride = _long_rows(q, "q", T, cols, dtype), _long_rows(out, "out", T, cols, dtype)
-    if not (table_stride > 0 and num_seqs >= 0 and 0 <= max_run < 2 ** 31 and 0 <= window < 2 ** 31):
-        raise ValueError("table_stride must be positive, num_seqs, max_run and window from 0 on and fit 32 bits")
+    if not (0 < table_stride < 2 ** 31 and num_seqs >= 0 and 0 <= max_run < 2 ** 31 and 0 <= window < 2 ** 31):
+        raise ValueError("table_stride must be positive, num_seqs, max_run and window from 0 on, and all fit 32 bits")
     _i32(run_start, "run_start", num_seqs + 1)
     _i32(seq_start, "seq_start", num_seqs)
     _i32(tables, "tables", num_seqs * table_stride)
