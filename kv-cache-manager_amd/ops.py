@@ -1279,7 +1279,7 @@ def rope_cache4(qkv, nh, nkv, hd, cache, slots, cos_sin=None, q_out=None, rows=N
     """Writes the k and v heads of the fused rows [q | k | v] to the slots (page * block_size + place, each at most once; one
     outside the pages, such as -1: kept nowhere) of a 4-bit cache (``cache4_shape``).  With a table of angles ``cos_sin`` (float32
     [rows, hd/2, 2]) k is rotated before, as ``rope_cache`` does, and q as well, to ``q_out`` [rows, nh * hd] (default: in its place
-    in ``qkv``); k and v of ``qkv`` stay as they are.  Without it nothing is rotated and q is not touched."""
+    in ``qkv``; otherwise memory that ``qkv`` does not use); k and v of ``qkv`` stay as they are.  Without it nothing is rotated and q is not touched."""
     T = qkv.shape[0] if rows is None else rows
     at, cache_at, slots_at, table_at, q_at = _one_gpu(qkv, cache, slots, cos_sin, q_out)
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
@@ -1339,7 +1339,8 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
     over the tokens 0 .. ctx_lens[r] - 1 of sequence row_seq[r] (``window`` > 0: the last ``window`` of them).  A row that sees nothing (a
     context of 0, a sequence without a table) gives zeros, and so would one whose pages all lie outside the cache: a table's entry that is
     no page hides its tokens.  ``max_context`` bounds every row's context length (what lies beyond it is not looked at) and decides how contexts are cut into parts that run side
-    by side, which needs ``scratch`` (attention_decode4_scratch floats; allocated here when not given)."""
+    by side, which needs ``scratch`` (attention_decode4_scratch floats; allocated here when not given).  Up to 65,535 rows; keys' and values'
+    ranges up to some 1e27, beyond which sums over them overflow."""
     T = q.shape[0] if rows is None else rows
     q_at, out_at, cache_at, tables_at, seq_at, lens_at, scratch_at = _one_gpu(q, out, cache, tables, row_seq, ctx_lens, scratch)
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
@@ -1372,7 +1373,7 @@ def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start
     """Causal attention over a 4-bit cache for runs of consecutive positions, as ``attention_prefill`` has them: sequence s owns rows
     run_start[s] .. run_start[s+1]-1, at most ``max_run``, the first of them at position seq_start[s]; every row sees the sequence's cached
     tokens up to its own position (``window`` > 0: the last ``window`` of them).  Rows of no run are left as they are.
-    ``max_context``: a bound of every row's context length (default: what the tables can hold)."""
+    ``max_context``: a bound of every row's context length (default: what the tables can hold).  Up to 65,535 sequences."""
     T = q.shape[0] if rows is None else rows
     q_at, out_at, cache_at, tables_at, run_at, start_at, scratch_at = _one_gpu(q, out, cache, tables, run_start, seq_start, scratch)
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)

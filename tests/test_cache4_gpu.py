@@ -588,3 +588,42 @@ def test_many_short_prompts(ops, nh, nkv, hd, seqs, dtype):
     some = list(range(0, T, 31)) + [T - 1]
     want, tol = s.expect(q[some], [seq[i] for i in some], [(0, pos[i] + 1) for i in some], hd ** -0.5)
     near(out[some], want, tol)
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+@pytest.mark.parametrize("nh, nkv, hd, page", ((64, 1, 64, 16), (33, 1, 32, 16), (40, 2, 128, 1008), (20, 1, 256, 16)))
+def test_many_heads_of_one_kv_head(ops, nh, nkv, hd, page, dtype):
+    gen = torch.Generator().manual_seed(nh)
+    lengths = (5, 1100, 64, 333)
+    s = Sequences(ops, nh, nkv, hd, page, lengths, gen, dtype)
+    q, out = queries(4, nh * hd, dtype, gen), torch.empty(4, nh * hd, dtype=dtype, device=DEV)
+    for window in (0, 50):
+        ops.attention_decode4(q, out, s.cache, s.dev_tables, s.stride, ints(range(4)), ints(lengths), nh, nkv, hd, hd ** -0.5, max(lengths), window=window)
+        want, tol = s.expect(q, range(4), [(max(0, n - window) if window else 0, n) for n in lengths], hd ** -0.5)
+        near(out, want, tol)
+
+
+def test_nothing_to_do(ops):
+    """No rows, no sequences, bounds of 0, runs that name rows and contexts that do not exist."""
+    nh, nkv, hd = 4, 2, 64
+    gen = torch.Generator().manual_seed(3)
+    s = Sequences(ops, nh, nkv, hd, 16, (40, 40), gen, BF)
+    q = queries(4, nh * hd, BF, gen)
+    nine = lambda: torch.full((4, nh * hd), 9.0, dtype=BF, device=DEV)
+    decode = lambda out, bound, **k: ops.attention_decode4(q, out, s.cache, s.dev_tables, s.stride, ints([0, 1, 0, 1]), ints([40, 3, 0, -2 ** 31]), nh, nkv, hd, 0.1, bound, **k)
+    prefill = lambda out, runs, starts, n, most, **k: ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints(runs), ints(starts), n, most, nh, nkv, hd, 0.1, **k)
+    for call in (lambda out: decode(out, 40, rows=0), lambda out: prefill(out, [0], [], 0, 4), lambda out: prefill(out, [0, 2, 4], [3, 3], 2, 0), lambda out: prefill(out, [2, 2, 2], [3, 3], 2, 4),
+                 lambda out: prefill(out, [4, 1, 0], [3, 3], 2, 4), lambda out: prefill(out, [7, 9, 2 ** 31 - 1], [3, 3], 2, 4)):
+        out = nine()
+        call(out)
+        assert bool((out == 9).all())
+    out = nine()
+    decode(out, 0)
+    assert not out.any()
+    out = nine()
+    prefill(out, [0, 2, 4], [-2 ** 31, -2], 2, 2)
+    assert not out.any()
+    out = nine()
+    prefill(out, [0, 1, 2 ** 31 - 1], [2 ** 31 - 1, 36], 2, 4, max_context=39)      # (rows 1 to 3: positions 36 to 38; row 0 sees what the bound allows)
+    want, tol = s.expect(q, [0, 1, 1, 1], [(0, 39), (0, 37), (0, 38), (0, 39)], 0.1)
+    near(out, want, tol)
