@@ -525,26 +525,34 @@ __global__ void __launch_bounds__(256) join4_kernel(const float* __restrict__ sc
   if (segs == 1) return;
   const size_t row = span.row0 + at;
   const float* left = scratch + (row * sh.nh + head) * sh.max_segs * (HD + 2);
-  float top = -FLT_MAX, sum = 0.f;
-  for (int i = threadIdx.x; i < segs; i += 256) top = fmaxf(top, left[i * (HD + 2) + HD]);
+  const int e = threadIdx.x % HD, g = threadIdx.x / HD;
+  const auto some_of = [&](int i, float (&next)[AHEAD]) {
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) next[n] = i + n * G < segs ? left[static_cast<size_t>(i + n * G) * (HD + 2) + e] : 0.f;
+  };
+  // the first ones are under way while the weights are made
+  float next[AHEAD];
+  some_of(g, next);
+  const int own = min(static_cast<int>(threadIdx.x), segs - 1) * (HD + 2) + HD;
+  const float own_m = left[own], own_l = left[own + 1];
+  float top = own_m, sum = 0.f;
+  for (int i = threadIdx.x + 256; i < segs; i += 256) top = fmaxf(top, left[i * (HD + 2) + HD]);
   top = wave_max(top);
   if (threadIdx.x % kWave == 0) of_wave[0][wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(of_wave[0][0], of_wave[0][1]), fmaxf(of_wave[0][2], of_wave[0][3]));
   for (int i = threadIdx.x; i < segs; i += 256) {
-    const float by = __builtin_amdgcn_exp2f(left[i * (HD + 2) + HD] - top);
+    const bool mine = i == static_cast<int>(threadIdx.x);
+    const float by = __builtin_amdgcn_exp2f((mine ? own_m : left[i * (HD + 2) + HD]) - top);
     weight[i] = by;
-    sum = fmaf(left[i * (HD + 2) + HD + 1], by, sum);
+    sum = fmaf(mine ? own_l : left[i * (HD + 2) + HD + 1], by, sum);
   }
   sum = wave_sum(sum);
   if (threadIdx.x % kWave == 0) of_wave[1][wave] = sum;
   __syncthreads();
-  const int e = threadIdx.x % HD, g = threadIdx.x / HD;
   float x = 0.f;
   for (int i = g; i < segs; i += AHEAD * G) {
-    float next[AHEAD];
-#pragma unroll
-    for (int n = 0; n < AHEAD; ++n) next[n] = i + n * G < segs ? left[static_cast<size_t>(i + n * G) * (HD + 2) + e] : 0.f;
+    if (i > g) some_of(i, next);
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) x = i + n * G < segs ? fmaf(next[n], weight[i + n * G], x) : x;
   }
