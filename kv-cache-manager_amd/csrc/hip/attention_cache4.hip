@@ -75,7 +75,6 @@ template <> constexpr int kTerms<float> = 3;
 template <class T> constexpr int kBias = 128;
 template <> constexpr int kBias<float> = 16;
 
-template <int N> struct Words { uint32_t w[N]; };
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   if constexpr (N == 1) {
@@ -619,7 +618,7 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   // Of 256 entries a CU holds four waves: two workgroups where there are enough (16 heads over 2: 200 rows of 300 tokens 11.7 us, with four
   // waves 16.4; a prompt of 2,048 91 and 108).
   if (parts == 1 && groups > 256 && hd == 256) p.waves = 2;
-  p.segment = static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
+  p.segment = parts == 1 ? LEAST : static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
   p.max_segs = parts == 1 ? 1 : static_cast<int>((static_cast<long long>(max_context) + p.segment - 1) / p.segment);
   if (parts > 1 && seen < max_context) p.max_segs = static_cast<int>((seen - 1) / p.segment + 2);
   p.floats = p.max_segs == 1 ? 0 : static_cast<long long>(T) * nh * p.max_segs * (hd + 2);
@@ -647,7 +646,8 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
   s.scale_log2 = scale * 1.4426950408889634f;
   s.window = window, s.max_context = static_cast<int>(std::min<long long>(static_cast<long long>(table_stride) * page, max_context));
   const long long x = static_cast<long long>(nkv) * p.max_segs * p.tiles;
-  KVCM_REQUIRE(x < (1ll << 30) && static_cast<long long>(rows.total) * (nh / nkv) < (1ll << 30) && units < 65536, "%s: %lld workgroups for each of %d sequences", what, x, units);
+  // (2^32 threads of a launch in x, at most 512 of a workgroup; quotients below 2^30)
+  KVCM_REQUIRE(x < (1ll << 23) && static_cast<long long>(rows.total) * (nh / nkv) < (1ll << 30) && units < 65536, "%s: %lld workgroups for each of %d sequences", what, x, units);
   KVCM_REQUIRE(p.max_segs == 1 || max_run < 65536, "%s: runs of %d rows cut into segments", what, max_run);
   const dim3 grid(static_cast<unsigned>(x), units);
   KVCM_HEAD4(hd, {

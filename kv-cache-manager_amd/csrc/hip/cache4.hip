@@ -194,7 +194,8 @@ int kvcm_rope_cache4(const void* qkv, int dtype, int stride, void* q_out, int q_
   KVCM_REQUIRE(qkv != nullptr && cache != nullptr && slots != nullptr && (cos_sin == nullptr || q_out != nullptr), "rope_cache4: null operand");
   const int first = cos_sin != nullptr ? 0 : nh, heads = nh + 2 * nkv - first;      // nothing rotates: the queries are not touched
   const long long vectors = static_cast<long long>(T) * heads, blocks = (vectors * (hd / 16) + kThreads - 1) / kThreads;
-  KVCM_REQUIRE(vectors < (1ll << 30) && blocks < (1ll << 30), "rope_cache4: %d rows of %d heads are too many for one launch", T, nh + 2 * nkv);
+  // (quotients below 2^30, 2^32 threads of a launch)
+  KVCM_REQUIRE(vectors < (1ll << 30) && blocks < (1ll << 24), "rope_cache4: %d rows of %d heads are too many for one launch", T, nh + 2 * nkv);
   KVCM_HEAD4(hd, {
     const auto go = [&](auto t) {
       using E = decltype(t);
@@ -217,7 +218,7 @@ int kvcm_cache4_rows(const void* cache, const int* slots, void* k, int k_stride,
   if (n == 0) return 0;
   KVCM_REQUIRE(cache != nullptr && slots != nullptr && k != nullptr && v != nullptr, "cache4_rows: null operand");
   const long long vectors = static_cast<long long>(n) * nkv, blocks = (vectors * (hd / 8) + kThreads - 1) / kThreads;
-  KVCM_REQUIRE(vectors < (1ll << 30) && blocks < (1ll << 30), "cache4_rows: %d tokens of %d heads are too many for one launch", n, nkv);
+  KVCM_REQUIRE(vectors < (1ll << 30) && blocks < (1ll << 24), "cache4_rows: %d tokens of %d heads are too many for one launch", n, nkv);
   KVCM_HEAD4(hd, {
     const auto go = [&](auto t) {
       using E = decltype(t);

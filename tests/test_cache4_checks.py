@@ -159,6 +159,9 @@ def test_numbers_that_do_not_fit_are_refused():
     assert lib.kvcm_attention_decode4(p, 1, 256, p, 256, p, p, 4, 2, p, p, 70000, 4, 2, 64, 9, 32, 0.1, 0, 100, 0, 0, 0) == -1 and "70000" in said()
     assert lib.kvcm_attention_prefill4(p, 1, 256, p, 256, p, p, 4, p, p, 2, 2 ** 30, 2 ** 30, 4, 2, 64, 9, 32, 0.1, 0, 100, 0, 0, 0) == -1 and "workgroups" in said()
     assert lib.kvcm_attention_decode4_scratch(1, 4, 2, 64, 2 ** 31 - 1, 2 ** 31 - 1) >= 0
+    assert lib.kvcm_rope_cache4(p, 1, 4096, 0, 0, p, p, 0, 2 ** 25, 8, 4, 256, 9, 32, 0) == -1 and "too many" in said()      # 2^32 threads and more
+    assert lib.kvcm_cache4_rows(p, p, p, 1024, p, 1024, 1, 2 ** 25, 4, 256, 9, 32, 0) == -1 and "too many" in said()
+    assert lib.kvcm_attention_prefill4(p, 1, 8192, p, 8192, p, p, 2 ** 22, p, p, 1, 2 ** 24, 2 ** 24, 32, 32, 256, 9, 32, 0.1, 0, 2 ** 24, 0, 0, 0) == -1 and "workgroups" in said()
 
 
 def test_operands_elsewhere_are_refused(monkeypatch):
