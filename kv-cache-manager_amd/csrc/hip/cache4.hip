@@ -73,23 +73,24 @@ __global__ void __launch_bounds__(kThreads) rope_cache4_kernel(const T* qkv, int
   const int at = blockIdx.x * (kThreads / G) + threadIdx.x / G;
   if (at >= vectors) return;      // all lanes of a vector together
   const int l = threadIdx.x % G, row = quotient(at, heads), head = at - row * heads.d + first;      // queries, keys, values
-  const bool value = head >= nh + nkv;
-  unsigned slot = 0;
-  if (head >= nh) {
-    slot = static_cast<unsigned>(slots[row]);
-    if (slot >= num_slots) return;      // -1: a padding row, nothing to keep
+  const bool value = head >= nh + nkv, turns = cos_sin != nullptr && !value;
+  // everything that is read is asked for before any of it is looked at
+  const unsigned slot = head >= nh ? static_cast<unsigned>(slots[row]) : 0u;
+  float4 angles[4] = {};
+  if (turns) {
+    const float4* from = reinterpret_cast<const float4*>(cos_sin + static_cast<size_t>(row) * (HD / 2) + 8 * l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) angles[i] = from[i];
   }
   float x[16];
   const T* src = qkv + static_cast<size_t>(row) * stride + head * HD + 8 * l;
   Eight<T>::load(src, x);
   Eight<T>::load(src + HD / 2, x + 8);
-  if (cos_sin != nullptr && !value) {
-    const float4* angles = reinterpret_cast<const float4*>(cos_sin + static_cast<size_t>(row) * (HD / 2) + 8 * l);
+  if (turns) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 u = angles[i];
-      rotate_in(x[2 * i], x[8 + 2 * i], u.x, u.y, T());
-      rotate_in(x[2 * i + 1], x[9 + 2 * i], u.z, u.w, T());
+      rotate_in(x[2 * i], x[8 + 2 * i], angles[i].x, angles[i].y, T());
+      rotate_in(x[2 * i + 1], x[9 + 2 * i], angles[i].z, angles[i].w, T());
     }
   }
   if (head < nh) {
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(kThreads) rope_cache4_kernel(const T* qkv, int
     Eight<T>::store(dst + HD / 2, x + 8);
     return;
   }
+  if (slot >= num_slots) return;      // -1: a padding row, nothing to keep
   float high = x[0], neg_low = -x[0], not_finite = x[0] * 0.f;
 #pragma unroll
   for (int i = 1; i < 16; ++i) {
