@@ -174,7 +174,7 @@ __device__ __forceinline__ uint32_t in_vector_register(uint32_t x) {
 // blockIdx.x: kv head (fastest: with eight of them each of the chip's eight parts keeps to one), then segment, then tile of rows, the last
 // tile first (it sees the most keys); blockIdx.y: token or sequence.
 constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what the registers are bounded for
-  return hd == 256 ? 1 : wide ? (rt == 1 ? 2 : 1) : hd == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 2;
+  return hd == 256 ? 1 : wide || rt == 2 ? 2 : hd == 128 ? 3 : 4;
 }
 template <class T, int HD, int RT, int W>
 __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
@@ -583,20 +583,30 @@ double expected_us(long long parts, long long groups, long long rounds, long lon
   return parts == 1 ? walk : walk + 2.5 + 0.07 * parts + static_cast<double>(T) * nh * (0.0008 + parts * (hd + 2) * 8 / 3e6);
 }
 
-Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
+Plan plan(bool wide, int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {
   Plan p{};
   const int group = nh / nkv;
   max_run = std::min(max_run, T);
   const long long pairs = static_cast<long long>(max_run) * group;
-  p.rt = pairs > 16 && hd <= 128 ? 2 : 1;
+  constexpr int LEAST = 4 * kChunk;      // tokens of a round: a chunk of each wave
+  long long groups, seen, rounds;
+  const auto tile = [&](int rt) {
+    p.rt = rt;
+    p.tile_rows = 16 * rt;
+    p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
+    groups = static_cast<long long>(units) * nkv * p.tiles;
+    seen = window > 0 ? std::min<long long>(static_cast<long long>(window) + p.tile_rows, max_context) : max_context;
+    rounds = (seen + LEAST - 1) / LEAST;
+  };
+  // Two tiles of rows to a wave share its operands; one tile leaves twice as many workgroups, and is the faster while there is work for less than
+  // two rounds of a full chip (32 heads over 8 of 128, one tile and two: four runs of 16 behind 500 tokens 7.2 us and 9.8, 16 of 64 behind 300
+  // 23.3 and 17.7; over 4 of 64: a prompt of 256 5.4 and 6.1, of 2,048 58 and 44).  Float rows, whose terms take the registers, always one (over 4 of
+  // 64, a prompt of 2,048 91 us and 94; over 8 of 128, three runs of 300 behind 4,000 211 and 276), and so 256 entries.
   p.waves = 4;
-  p.tile_rows = 16 * p.rt;
-  p.tiles = static_cast<int>((pairs + p.tile_rows - 1) / p.tile_rows);
-  const long long groups = static_cast<long long>(units) * nkv * p.tiles;
-  const long long seen = window > 0 ? std::min<long long>(static_cast<long long>(window) + p.tile_rows, max_context) : max_context;
+  tile(pairs > 16 && hd <= 128 && !wide ? 2 : 1);
+  if (p.rt == 2 && groups * rounds < 2 * kFill) tile(1);
   // How many parts contexts are cut into: what the model makes least, among 1 2 3 4 6 8 12 16 .. and what fills the chip once.
-  constexpr int LEAST = 4 * kChunk;      // a chunk of each wave
-  const long long rounds = (seen + LEAST - 1) / LEAST, most = std::min(2 * kFill / groups, rounds);
+  const long long most = std::min(2 * kFill / groups, rounds);
   long long parts = 1;
   double least = expected_us(1, groups, rounds, T, nh, hd);
   const auto consider = [&](long long n) {
@@ -625,6 +635,10 @@ Plan plan(int units, int T, int max_run, int nh, int nkv, int hd, int max_contex
   return p;
 }
 
+long long scratch_floats(int units, int T, int max_run, int nh, int nkv, int hd, int max_context, int window) {      // for rows of either type
+  return std::max(plan(false, units, T, max_run, nh, nkv, hd, max_context, window).floats, plan(true, units, T, max_run, nh, nkv, hd, max_context, window).floats);
+}
+
 int launch(const char* what, const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride, Rows rows,
            int units, int max_run, int nh, int nkv, int hd, int pages, int page, float scale, int window, int max_context, float* scratch, long long scratch_floats,
            hipStream_t stream) {
@@ -637,7 +651,7 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
   KVCM_REQUIRE(rows.total > 0 && max_run > 0, "%s: %d rows, runs of up to %d", what, rows.total, max_run);
   KVCM_REQUIRE(q != nullptr && out != nullptr && cache != nullptr && tables != nullptr && rows.where != nullptr && rows.lens != nullptr, "%s: null operand", what);
   max_run = std::min(max_run, rows.total);
-  const Plan p = plan(units, rows.total, max_run, nh, nkv, hd, max_context, window);
+  const Plan p = plan(dtype == kF32, units, rows.total, max_run, nh, nkv, hd, max_context, window);
   KVCM_REQUIRE(p.floats == 0 || (scratch != nullptr && scratch_floats >= p.floats), "%s: scratch of %lld floats is needed", what, p.floats);
   Shape s{};
   s.q_stride = q_stride, s.out_stride = out_stride, s.table_stride = table_stride, s.nh = nh, s.pages = pages;
@@ -662,7 +676,7 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       constexpr std::integral_constant<int, 1> one;
       constexpr std::integral_constant<int, 4> four;
       constexpr std::integral_constant<int, 2> two;
-      constexpr std::integral_constant<int, HD == 256 ? 1 : 2> most;
+      constexpr std::integral_constant<int, HD == 256 || sizeof(T) == 4 ? 1 : 2> most;
       if (p.rt == 2 && p.waves == 2) walk(most, two);
       else if (p.rt == 2) walk(most, four);
       else if (p.waves == 2) walk(one, two);
@@ -685,7 +699,7 @@ extern "C" {
 
 long long kvcm_attention_decode4_scratch(int T, int nh, int nkv, int hd, int max_context, int window) {
   if (T <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0) return 0;
-  return plan(T, T, 1, nh, nkv, hd, max_context, window).floats;
+  return scratch_floats(T, T, 1, nh, nkv, hd, max_context, window);
 }
 
 int kvcm_attention_decode4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride, int seqs,
@@ -698,7 +712,7 @@ int kvcm_attention_decode4(const void* q, int dtype, int q_stride, void* out, in
 
 long long kvcm_attention_prefill4_scratch(int T, int nh, int nkv, int hd, int max_context, int max_run, int num_seqs, int window) {
   if (T <= 0 || nkv <= 0 || nh <= 0 || nh % nkv != 0 || max_run <= 0 || num_seqs <= 0) return 0;
-  return plan(num_seqs, T, max_run, nh, nkv, hd, max_context, window).floats;
+  return scratch_floats(num_seqs, T, max_run, nh, nkv, hd, max_context, window);
 }
 
 int kvcm_attention_prefill4(const void* q, int dtype, int q_stride, void* out, int out_stride, const void* cache, const int* tables, int table_stride,
