@@ -574,7 +574,7 @@ def test_many_rows_of_short_contexts(ops, nh, nkv, hd, rows, dtype):
         near(out[some], want, tol)
 
 
-@pytest.mark.parametrize("nh, nkv, hd, seqs, dtype", ((32, 4, 64, 40, BF), (8, 8, 128, 60, BF), (16, 2, 32, 70, F32), (8, 1, 256, 40, BF)))
+@pytest.mark.parametrize("nh, nkv, hd, seqs, dtype", ((32, 4, 64, 40, BF), (8, 8, 128, 60, BF), (16, 2, 32, 70, F32), (16, 2, 32, 70, BF), (8, 1, 256, 40, BF)))
 def test_many_short_prompts(ops, nh, nkv, hd, seqs, dtype):
     gen = torch.Generator().manual_seed(seqs + hd)
     runs = torch.randint(1, 70, (seqs,), generator=gen).tolist()
@@ -627,3 +627,25 @@ def test_nothing_to_do(ops):
     prefill(out, [0, 1, 2 ** 31 - 1], [2 ** 31 - 1, 36], 2, 4, max_context=39)      # (rows 1 to 3: positions 36 to 38; row 0 sees what the bound allows)
     want, tol = s.expect(q, [0, 1, 1, 1], [(0, 39), (0, 37), (0, 38), (0, 39)], 0.1)
     near(out, want, tol)
+
+
+@pytest.mark.parametrize("nh, nkv, hd, runs, starts, window, dtype", (
+    (32, 4, 64, (1100,), (0,), 0, BF), (32, 4, 64, (700, 555), (30, 0), 200, BF), (16, 2, 32, (1500, 600), (0, 77), 0, BF), (8, 8, 128, (900, 1000), (200, 0), 0, BF),
+    (32, 4, 64, (64,), (8000,), 0, BF), (8, 2, 128, (130, 99), (8000, 5000), 0, BF), (8, 2, 128, (300, 299), (3000, 2500), 2500, BF), (32, 4, 32, (90,), (7000,), 0, BF),
+    (32, 4, 64, (500, 333), (200, 0), 0, F32), (16, 2, 256, (600, 300), (0, 100), 0, BF)))
+def test_long_runs(ops, nh, nkv, hd, runs, starts, window, dtype):
+    gen = torch.Generator().manual_seed(sum(runs) + hd)
+    s = Sequences(ops, nh, nkv, hd, 16, [r + p for r, p in zip(runs, starts)], gen, dtype)
+    first = np.concatenate([[0], np.cumsum(runs)])
+    T = int(first[-1])
+    q, out = queries(T, nh * hd, dtype, gen), torch.full((T, nh * hd), 9.0, dtype=dtype, device=DEV)
+    args = (q, out, s.cache, s.dev_tables, s.stride, ints(first), ints(starts), len(runs), max(runs), nh, nkv, hd, hd ** -0.5)
+    ops.attention_prefill4(*args, window=window)
+    seq, pos = [i for i, r in enumerate(runs) for _ in range(r)], [p + j for r, p in zip(runs, starts) for j in range(r)]
+    some = sorted(set(range(0, T, T // 40)) | {0, 1, 2, 3, 4, T - 2, T - 1})
+    want, tol = s.expect(q[some], [seq[i] for i in some], [(max(0, pos[i] + 1 - window) if window else 0, pos[i] + 1) for i in some], hd ** -0.5)
+    near(out[some], want, tol)
+    assert not bool(out.isnan().any())
+    again = out.clone()
+    ops.attention_prefill4(*args, window=window)
+    assert torch.equal(again, out)
