@@ -1329,9 +1329,13 @@ def _scratch4(what, need, scratch, device):
 
 
 @functools.lru_cache(maxsize=4096)
+def _decode4_floats(*sizes):
+    return int(lib().kvcm_attention_decode4_scratch(*sizes))
+
+
 def attention_decode4_scratch(rows, nh, nkv, hd, max_context, window=0):
     """Floats of scratch ``attention_decode4`` needs for these sizes (0: contexts are not cut)."""
-    return int(lib().kvcm_attention_decode4_scratch(rows, nh, nkv, hd, int(max_context), int(window)))
+    return _decode4_floats(int(rows), int(nh), int(nkv), int(hd), int(max_context), int(window))
 
 
 def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh, nkv, hd, scale, max_context, scratch=None, window=0, rows=None):
@@ -1363,9 +1367,13 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
 
 
 @functools.lru_cache(maxsize=4096)
+def _prefill4_floats(*sizes):
+    return int(lib().kvcm_attention_prefill4_scratch(*sizes))
+
+
 def attention_prefill4_scratch(rows, nh, nkv, hd, max_context, max_run, num_seqs, window=0):
     """Floats of scratch ``attention_prefill4`` needs for a launch of these sizes (0: contexts are not cut)."""
-    return int(lib().kvcm_attention_prefill4_scratch(rows, nh, nkv, hd, int(max_context), max_run, num_seqs, int(window)))
+    return _prefill4_floats(int(rows), int(nh), int(nkv), int(hd), int(max_context), int(max_run), int(num_seqs), int(window))
 
 
 def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start, num_seqs, max_run, nh, nkv, hd, scale, rows=None,

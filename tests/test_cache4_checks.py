@@ -182,3 +182,11 @@ def test_scratch_of_any_size_is_bounded(nh, nkv, hd):
                 assert ctx > 256 or floats == 0
                 runs = ops.attention_prefill4_scratch(rows, nh, nkv, hd, ctx, rows, 1, window)
                 assert 0 <= runs <= rows * nh * (1536 // nkv + 2) * (hd + 2)
+
+
+def test_scratch_goes_by_values():
+    """Sizes may be anything that counts, and what they come to is never a former call's."""
+    size = torch.tensor(100)
+    assert ops.attention_decode4_scratch(1, 32, 8, 128, size) == 0
+    size += 30000
+    assert ops.attention_decode4_scratch(1, 32, 8, 128, size) == ops.attention_decode4_scratch(1, 32, 8, 128, 30100) > 0
