@@ -1296,6 +1296,12 @@ def rope_cache4(qkv, nh, nkv, hd, cache, slots, cos_sin=None, q_out=None, rows=N
             q_at, q_stride = at, stride
         else:
             q_stride = _long_rows(q_out, "q_out", T, nh * hd, dtype)
+            wide, own, size = (nh + 2 * nkv) * hd, nh * hd, 2 if dtype is torch.bfloat16 else 4
+            if q_at < at + (T * stride - stride + wide) * size and at < q_at + (T * q_stride - q_stride + own) * size:
+                # the rows' own queries, or beside them in wider rows: anything else would be written before it has been read
+                shift = (q_at - at) // size % stride
+                if not (q_at == at and (T <= 1 or q_stride == stride) or q_stride == stride and wide <= shift <= stride - own):
+                    raise ValueError("q_out must be the rows' own queries or memory that qkv does not use")
     _call("kvcm_rope_cache4", at, _DT[dtype], stride, q_at, q_stride, cache_at, slots_at, table_at, T, nh, nkv, hd, pages, page, _stream())
 
 

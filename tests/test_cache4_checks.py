@@ -190,3 +190,26 @@ def test_scratch_goes_by_values():
     assert ops.attention_decode4_scratch(1, 32, 8, 128, size) == 0
     size += 30000
     assert ops.attention_decode4_scratch(1, 32, 8, 128, size) == ops.attention_decode4_scratch(1, 32, 8, 128, 30100) > 0
+
+
+def test_queries_written_over_rows_that_are_still_read_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_one_gpu", lambda *tensors: [0 if t is None else t.data_ptr() for t in tensors])
+    monkeypatch.setattr(ops, "_call", lambda *args: None)
+    wide = (NH + 2 * NKV) * HD
+    for dtype in (BF, F32):
+        held = torch.zeros(T + 2, wide + NH * HD + 7, dtype=dtype)
+        rest = dict(slots=torch.zeros(T, dtype=I32), cos_sin=torch.zeros(T, HD // 2, 2), cache=torch.zeros(ops.cache4_shape(PAGES, NKV, HD, PAGE), dtype=U8), rows=T)
+        rows, behind = held[:T, :wide], held[:T, NH * HD + 7:]
+        store(qkv=rows, q_out=rows[:, :NH * HD], **rest)
+        store(qkv=rows, q_out=rows, **rest)
+        store(qkv=rows, q_out=held[:T, wide:], **rest)
+        store(qkv=rows, q_out=held[:T, wide + 7:], **rest)
+        store(qkv=behind, q_out=held[:T, :NH * HD], **rest)
+        store(qkv=behind, q_out=held[:T, 7:], **rest)
+        store(qkv=rows, q_out=torch.zeros(T, NH * HD, dtype=dtype), **rest)
+        store(qkv=rows, q_out=held.view(-1)[:T * NH * HD].view(T, -1)[:1], **rest | dict(rows=1))
+        for bad in (rows[:, 1:], rows[:, HD:], held[1:T + 1, :wide], held[:T, wide - 1:], held.view(-1)[:T * NH * HD].view(T, -1), held[:T, 7:]):
+            with pytest.raises(ValueError, match="q_out must be the rows"):
+                store(qkv=rows, q_out=bad, **rest)
+        with pytest.raises(ValueError, match="q_out must be the rows"):
+            store(qkv=behind, q_out=held[:T, 8:], **rest)
