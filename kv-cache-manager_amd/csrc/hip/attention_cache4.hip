@@ -8,18 +8,22 @@
 // so that the scores of a lane all belong to one row (lane % 16) and are, as they stand, what the second product takes from that
 // lane.  Nothing passes through LDS.
 //
-// Codes become operands without arithmetic: in bfloat16 0x4300 | c is 128 + c and 0x4180 | c << 3 is 16 + c, exactly, and one shift and one
-// bit operation give two of them (7 or 8 instructions for 8 codes; keys and values both lie in the order that this needs).  Rows of
-// bfloat16 take B = 128, float rows, whose 32 bits the larger numbers would eat into, B = 16.  With f the scale times log2 e,
+// Codes become operands without arithmetic: in bfloat16 0x4180 | c << 3 is B + c with B = 16, exactly, and one shift and one bit operation
+// give two of them (8 instructions for 8 codes; keys and values both lie in the order that this needs).  0x4300 | c, 128 + c, spares one of
+// the eight, 1 to 3 % of the time (6 % of prompts with 256 entries), but sums 5 times as large lose as much more of their 32 bits: with keys
+// and queries of 20 +- 20 a score was off by up to 0.06 at 128 entries and 0.1 at 256, and is by 0.005 and 0.008.  With f the scale times
+// log2 e,
 //   f q . k - m = (f step) (q . (B + c)) + [low (f sum q) - B step (f sum q) - m]
 // where the bracket is a matrix instruction of its own, m its accumulator's start: a pair (step, low) as it lies in the cache is an
-// operand, against f sum q as three bfloat16 numbers (24 bits) and -B times them.  (Float rows: q . (B + c) - (B + 8) sum q comes first,
-// the small terms of q before the large, and 8 step in the bracket: sums stay as small as what they come to.)  One multiplication and
-// addition for each score leaves the exponential's argument.
+// operand, against f sum q as three bfloat16 numbers (24 bits) and -B times them.  (Float rows and 128 entries or more: q . (B + c) starts
+// from -(B + 8) sum q, with the small terms of float queries before the large, and 8 step is in the bracket: sums stay nearer to what they
+// come to.)  One multiplication and addition for each score leaves the exponential's argument.
 //   sum p v = sum (p step) (B + c) - (B + 8) sum (p step) + sum p (low + 8 step)
-// where p step is what is rounded to bfloat16 (float rows: split into three, which keep all 24 bits, as q is), and its sum comes from
-// one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0
-// as the values are from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
+// where p step is what is rounded to bfloat16, as attention over the 16-bit cache rounds p: a second term would double the matrix work over
+// values for a part of the error that is less than the rounded output's own (normal keys and values, 1,000 tokens: 2.3e-3 of the output's norm,
+// 1.65e-3 if nothing but the output were rounded).  Float rows split it into three, which keep all 24 bits, as q is.  Its sum comes
+// from one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is
+// multiplied with is c - 8, as far from 0 as the values are from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
 //
 // m is not the largest score but one that no score passes by more than 2^6: it moves in few chunks, and only then do a row's four lanes
 // compare what they have and the sums get scaled.
@@ -58,12 +62,9 @@ __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
 }
 // B + c of the codes 4s .. 4s + 3 bits into either half of a word: one bit operation takes the mask and B, where one of them lies in a vector
 // register (`mask`; an instruction reads one scalar register).
-template <int B> constexpr uint32_t kMask = B == 128 ? 0x000F000Fu : 0x00780078u;
-template <int B>
-__device__ __forceinline__ uint32_t codes(uint32_t word, int s, uint32_t mask) {
-  if constexpr (B == 128) return (word >> (4 * s) & mask) | 0x43004300u;
-  return ((s == 0 ? word << 3 : word >> (4 * s - 3)) & mask) | 0x41804180u;
-}
+constexpr int B = 16;
+constexpr uint32_t kMask = 0x00780078u;
+__device__ __forceinline__ uint32_t codes(uint32_t word, int s, uint32_t mask) { return ((s == 0 ? word << 3 : word >> (4 * s - 3)) & mask) | 0x41804180u; }
 
 // The low halves of two words side by side, and the high ones.
 __device__ __forceinline__ uint32_t pick_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
@@ -72,8 +73,9 @@ __device__ __forceinline__ uint32_t pick_high(uint32_t a, uint32_t b) { return _
 // Numbers as sums of bfloat16 ones: one for rows of bfloat16, three for float (24 bits).
 template <class T> constexpr int kTerms = 1;
 template <> constexpr int kTerms<float> = 3;
-template <class T> constexpr int kBias = 128;
-template <> constexpr int kBias<float> = 16;
+// Whether the sum over a key's codes starts from -(B + 8) sum q.  Bfloat16 rows of fewer than 128 entries have shorter sums and need the start's
+// registers more (64 entries, a prompt of 2,048: two waves to a SIMD instead of three, 48.7 us and 41.9; 128 entries: 63.6 and 63.7).
+template <class T, int HD> constexpr bool kFromMiddle = kTerms<T> > 1 || HD >= 128;
 
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
@@ -179,7 +181,8 @@ constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what t
 template <class T, int HD, int RT, int W>
 __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
                                                               const int* __restrict__ tables, Rows rows, Shape sh, float* __restrict__ scratch) {
-  constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>, B = kBias<T>;
+  constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>;
+  constexpr bool MID = kFromMiddle<T, HD>;
   const int rest = quotient(blockIdx.x, sh.nkv), kvh = blockIdx.x - rest * sh.nkv.d, tile_up = quotient(rest, sh.segs), part = rest - tile_up * sh.max_segs;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, n16 = lane % 16, kq = lane / 16;
   const int group = sh.group.d;
@@ -234,13 +237,13 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
       for (int c = 0; c < KS; ++c) sums = product(ones, qf[rt][n][c], sums);
     const float sum = sums[0];
     const float less = -(B + 8.f) * sum;
-    start[rt] = f32x4{less, less, less, less};      // (float rows)
+    start[rt] = f32x4{less, less, less, less};
     // against a pair (step, low), three times: what step and low are multiplied with (the first lane of a row; the others' is 0)
     float left = kq == 0 ? sum * sh.scale_log2 : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float term = i < 3 ? round_to<bf16_t>(left) : 0.f;
-      q_sum[rt][i] = pack((NT == 1 ? -B : 8.f) * term, term);
+      q_sum[rt][i] = pack((MID ? 8.f : -B) * term, term);
       left -= term;
     }
   }
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
   const int* table = tables + static_cast<size_t>(max(span.seq, 0)) * sh.table_stride;      // (looked at only where there are tokens)
   const int k_at = n16 * (HD / 2) + kq * (HD / 8), v_at = value4_at(HD) + (kq * 16 + n16) * (HD / 8);
   const int kp_at = 8 * HD + kq * 16, vp_at = value4_at(HD) + 8 * HD + kq * 16, token_at = 8 * HD + n16 * 4;
-  const uint32_t mask = in_vector_register(kMask<B>);
+  const uint32_t mask = in_vector_register(kMask);
 
   // Of either tile of a chunk: where it lies, and whether it has tokens.  One past the end stands for the last, one whose page is none for
   // the cache's first page (nobody looks at their tokens): no load and no address is behind a branch.
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     for (int j = 0; j < 2; ++j) {
       u32x4 kf[KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) kf[k] = u32x4{codes<B>(c.k[j][k], 0, mask), codes<B>(c.k[j][k], 1, mask), codes<B>(c.k[j][k], 2, mask), codes<B>(c.k[j][k], 3, mask)};
+      for (int k = 0; k < KS; ++k) kf[k] = u32x4{codes(c.k[j][k], 0, mask), codes(c.k[j][k], 1, mask), codes(c.k[j][k], 2, mask), codes(c.k[j][k], 3, mask)};
       const u32x4 pairs{c.of_token[j], c.of_token[j], c.of_token[j], c.of_token[j]};
       float step[4];
 #pragma unroll
@@ -313,13 +316,12 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
       for (int rt = 0; rt < RT; ++rt) {
         const f32x4 rest = product(pairs, q_sum[rt], less_m[rt]);
         f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if constexpr (NT > 1) {
 #pragma unroll
-          for (int n = NT - 1; n > 0; --n)
+        for (int n = NT - 1; n > 0; --n)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) x = product(kf[k], qf[rt][n][k], x);
-          x += start[rt];
-        }
+          for (int k = 0; k < KS; ++k) x = product(kf[k], qf[rt][n][k], x);
+        if constexpr (NT > 1) x += start[rt];
+        else if constexpr (MID) x = start[rt];
 #pragma unroll
         for (int k = 0; k < KS; ++k) x = product(kf[k], qf[rt][0][k], x);
 #pragma unroll
@@ -406,8 +408,8 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int pair = 0; pair < 2; ++pair) {
-          if constexpr (C == 2) vf[2 * j + pair] = codes<B>(c.v[j][0], d + 2 * pair, mask);
-          else vf[2 * j + pair] = codes<B>(c.v[j][pair * (C / 4) + d / 4], d % 4, mask);
+          if constexpr (C == 2) vf[2 * j + pair] = codes(c.v[j][0], d + 2 * pair, mask);
+          else vf[2 * j + pair] = codes(c.v[j][pair * (C / 4) + d / 4], d % 4, mask);
         }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)

@@ -649,3 +649,37 @@ def test_long_runs(ops, nh, nkv, hd, runs, starts, window, dtype):
     again = out.clone()
     ops.attention_prefill4(*args, window=window)
     assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("nh, hd, rows", ((1, 32, 400), (1, 64, 400), (1, 128, 400), (1, 256, 400), (32, 64, 1600), (32, 128, 1600)))
+@pytest.mark.parametrize("dtype", (BF, F32))
+def test_scores_of_far_off_entries_stay_exact(ops, dtype, nh, hd, rows):
+    """Two tokens whose scores are nearly alike, of keys and queries around 20: the value of one is 1 everywhere and of the other -1 (step 0,
+    nothing of p is rounded), so that the output is tanh of half the scores' difference and its error half the scores'.
+
+    What the scores may be off by, root of the mean square: a sum over hd entries comes about in hd / 32 matrix instructions, the j-th of them
+    at no more than j 32 / hd of (16 + 8) sum|q|, and is multiplied with step * scale; each rounds by up to u = 2^-24 of what it holds, evenly (so
+    u / sqrt 3).  Two roundings more at up to two thirds of that for the terms beside it (16 step and low, times sum q).  Twice all this, for
+    instructions that cut where others round; two tokens; half of it in the output, which is rounded itself (at most half a unit in its last place)."""
+    gen = torch.Generator().manual_seed(hd + nh)
+    x = torch.randn(2, 3 * hd, generator=gen) * 20 + 20
+    x[0, 2 * hd:], x[1, 2 * hd:] = 1, -1
+    cache = torch.zeros(ops.cache4_shape(1, 1, hd, 16), dtype=torch.uint8, device=DEV)
+    ops.rope_cache4(x.to(dtype).to(DEV), 1, 1, hd, cache, ints(range(2)))
+    kc, ks, kl, _, vs, vl = plain.parts(cache, 1, hd)
+    assert not vs[:2].any() and vl[0, 0] == 1 and vl[1, 0] == -1
+    k, scale = (kl + ks * kc)[:2, 0], hd ** -0.5
+    q = torch.randn(rows * nh, hd, generator=gen).double().to(DEV) * 20 + 20
+    between = k[0] - k[1]
+    q = (q - (q @ between / (between @ between)).view(-1, 1) * between).to(dtype)
+    s = q.double() @ k.T * scale
+    want = torch.tanh((s[:, 0] - s[:, 1]) / 2)
+    out = torch.empty(rows, nh * hd, dtype=dtype, device=DEV)
+    ops.attention_decode4(q.view(rows, -1), out, cache, ints([0]), 1, ints([0] * rows), ints([2] * rows), nh, 1, hd, scale, 2)
+    off = out.view(rows * nh, hd).double() - want.view(-1, 1)
+    u, n = 2.0 ** -24, hd // 32
+    held = 24 * q.double().abs().sum(1) * ks[:2].max() * scale
+    scores = 2 * (2 * (sum((j / n) ** 2 for j in range(1, n + 1)) + 2 * (2 / 3) ** 2)) ** 0.5 * u / 3 ** 0.5 * held
+    tol = scores / 2 + torch.finfo(dtype).eps / 2 * want.abs()
+    rms = lambda v: float(v.square().mean().sqrt())
+    assert rms(off) <= rms(tol), (rms(off), rms(tol))
