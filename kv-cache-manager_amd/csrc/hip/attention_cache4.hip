@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     for (int d = 0; d < C; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int chunk_first = lo / kChunk + wave, chunk_end = (hi + kChunk - 1) / kChunk;      // every W-th of them
+  const int chunk_first = lo / kChunk + wave, chunk_end = (static_cast<unsigned>(hi) + kChunk - 1) / kChunk;      // every W-th of them
   const int* table = tables + static_cast<size_t>(max(span.seq, 0)) * sh.table_stride;      // (looked at only where there are tokens)
   const int k_at = n16 * (HD / 2) + kq * (HD / 8), v_at = value4_at(HD) + (kq * 16 + n16) * (HD / 8);
   const int kp_at = 8 * HD + kq * 16, vp_at = value4_at(HD) + 8 * HD + kq * 16, token_at = 8 * HD + n16 * 4;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     Ids ids = ids_of(chunk), next = ids_of(chunk + W);
     request_keys(ids, c);
     request_values(ids, c);
-    const int whole_lo = max(all_lo, lo), whole_hi = min(all_hi, hi);
+    const unsigned whole_lo = max(all_lo, lo), whole_hi = min(all_hi, hi);
     const auto take = [&](auto whole) {
       const Ids after = ids_of(chunk + 2 * W);
       score(c, s);
@@ -443,7 +443,10 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
       ids = next;
       next = after;
     };
-    const auto all_see = [&] { return chunk * kChunk >= whole_lo && (chunk + 1) * kChunk <= whole_hi && ids.some[0] && ids.some[1]; };
+    const auto all_see = [&] {      // (the chunk's end may be 2^31)
+      const unsigned t = static_cast<unsigned>(chunk) * kChunk;
+      return t >= whole_lo && t + kChunk <= whole_hi && ids.some[0] && ids.some[1];
+    };
     while (chunk < chunk_end) {
       while (all_see()) take(std::true_type());
       if (chunk < chunk_end) take(std::false_type());

@@ -683,3 +683,21 @@ def test_scores_of_far_off_entries_stay_exact(ops, dtype, nh, hd, rows):
     tol = scores / 2 + torch.finfo(dtype).eps / 2 * want.abs()
     rms = lambda v: float(v.square().mean().sqrt())
     assert rms(off) <= rms(tol), (rms(off), rms(tol))
+
+
+@pytest.mark.parametrize("window", (20, 0))
+def test_the_longest_context_that_slots_can_number(ops, window):
+    """A context of 2^31 - 16 tokens, all of whose pages but the last two are none: the tokens at its end are seen."""
+    nh, nkv, hd, page, n = 2, 1, 32, 16, 2 ** 31 - 16
+    gen = torch.Generator().manual_seed(51)
+    cache = filled(ops, 5, nkv, hd, page, gen, list(range(80)))
+    tables = torch.full((n // page,), -1, dtype=torch.int32, device=DEV)
+    tables[-2:] = ints([3, 1])
+    q, out = queries(1, nh * hd, BF, gen), torch.full((1, nh * hd), 9.0, dtype=BF, device=DEV)
+    slots = torch.cat([torch.arange(48, 64, device=DEV), torch.arange(16, 32, device=DEV)])
+    want, tol = plain.attend(q.double().view(1, nh, hd), plain.parts(cache, nkv, hd), [slots], [(32 - window if window else 0, 32)], nh, nkv, 0.2, BF)
+    ops.attention_decode4(q, out, cache, tables, n // page, ints([0]), ints([n]), nh, nkv, hd, 0.2, n, window=window)
+    near(out, want, tol)
+    out.fill_(9.0)
+    ops.attention_prefill4(q, out, cache, tables, n // page, ints([0, 1]), ints([n - 1]), 1, 1, nh, nkv, hd, 0.2, max_context=n, window=window)
+    near(out, want, tol)
