@@ -132,8 +132,8 @@ __device__ __forceinline__ Span span_of(const Rows& r, const Shape& s, int unit)
 // Tokens that position i of a span sees: [first, end).
 __device__ __forceinline__ int end_of(const Span& p, const Shape& s, int i) { return max(0, min(p.ctx0 + i + 1, s.max_context)); }
 __device__ __forceinline__ int first_of(const Span& p, const Shape& s, int i) {
-  const int end = end_of(p, s, i);
-  return s.window > 0 ? max(0, min(end, p.ctx0 + i + 1 - s.window)) : 0;
+  const int end = end_of(p, s, i), ctx = p.ctx0 + i + 1;      // (below 0 for a run that begins in front of its sequence)
+  return s.window > 0 && ctx > s.window ? min(end, ctx - s.window) : 0;
 }
 
 // Which segments the tokens of a tile of rows lie in.

@@ -701,3 +701,16 @@ def test_the_longest_context_that_slots_can_number(ops, window):
     out.fill_(9.0)
     ops.attention_prefill4(q, out, cache, tables, n // page, ints([0, 1]), ints([n - 1]), 1, 1, nh, nkv, hd, 0.2, max_context=n, window=window)
     near(out, want, tol)
+
+
+def test_runs_in_front_of_their_sequence_see_nothing(ops):
+    """Rows at positions below 0, down to the smallest, under windows of any size: zeros; the run's rows from position 0 on as ever."""
+    nh, nkv, hd = 4, 2, 64
+    gen = torch.Generator().manual_seed(52)
+    s = Sequences(ops, nh, nkv, hd, 16, (40, 40), gen, BF)
+    q = queries(6, nh * hd, BF, gen)
+    for window in (0, 1, 2 ** 31 - 1):
+        out = torch.full((6, nh * hd), 9.0, dtype=BF, device=DEV)
+        ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints([0, 2, 6]), ints([-2 ** 31, -2]), 2, 4, nh, nkv, hd, 0.1, window=window)
+        want, tol = s.expect(q, [-1, -1, 1, 1, 1, 1], [(0, 0)] * 4 + [(0, 1), (1, 2) if window == 1 else (0, 2)], 0.1)
+        near(out, want, tol)
