@@ -1272,6 +1272,8 @@ def _long_rows(t, name, rows, cols, dtype):
         raise ValueError(f"{name} must be {dtype if dtype in _DT else 'bfloat16 or float32'}")
     if not (s[0] >= rows >= 0 and s[1] >= cols and (st[0] >= cols or rows <= 1) and st[0] < 2 ** 31):
         raise ValueError(f"{name} must be [>= {rows}, >= {cols}] with rows of their own")
+    if rows >= 2 ** 31 or cols >= 2 ** 31:
+        raise ValueError(f"{name}: {rows} rows of {cols} entries do not fit 32 bits")
     return max(st[0], cols)
 
 
@@ -1362,13 +1364,16 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
     _i32(tables, "tables")
     if not held >= table_stride > 0:
         raise ValueError("tables must hold rows of table_stride pages")
+    tables_held = held // table_stride
+    if not (table_stride < 2 ** 31 and tables_held < 2 ** 31):
+        raise ValueError("table_stride and the number of tables must fit 32 bits")
     if not (0 <= window < 2 ** 31 and 0 <= max_context < 2 ** 31):
         raise ValueError("window and max_context must be from 0 on and fit 32 bits")
     need, floats = attention_decode4_scratch(T, nh, nkv, hd, max_context, window), 0
     if need or scratch is not None:
         scratch, floats = _scratch4("attention_decode4", need, scratch, q.device)
         scratch_at = scratch.data_ptr()
-    _call("kvcm_attention_decode4", q_at, _DT[dtype], q_stride, out_at, out_stride, cache_at, tables_at, table_stride, held // table_stride, seq_at,
+    _call("kvcm_attention_decode4", q_at, _DT[dtype], q_stride, out_at, out_stride, cache_at, tables_at, table_stride, tables_held, seq_at,
           lens_at, T, nh, nkv, hd, pages, page, float(scale), int(window), int(max_context), scratch_at, floats, _stream())
 
 
@@ -1393,7 +1398,7 @@ def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
     dtype, cols = q.dtype, nh * hd
     q_stride, out_stride = _long_rows(q, "q", T, cols, dtype), _long_rows(out, "out", T, cols, dtype)
-    if not (0 < table_stride < 2 ** 31 and num_seqs >= 0 and 0 <= max_run < 2 ** 31 and 0 <= window < 2 ** 31):
+    if not (0 < table_stride < 2 ** 31 and 0 <= num_seqs < 2 ** 31 and 0 <= max_run < 2 ** 31 and 0 <= window < 2 ** 31):
         raise ValueError("table_stride must be positive, num_seqs, max_run and window from 0 on, and all fit 32 bits")
     _i32(run_start, "run_start", num_seqs + 1)
     _i32(seq_start, "seq_start", num_seqs)

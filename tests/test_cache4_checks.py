@@ -213,3 +213,19 @@ def test_queries_written_over_rows_that_are_still_read_are_refused(monkeypatch):
                 store(qkv=rows, q_out=bad, **rest)
         with pytest.raises(ValueError, match="q_out must be the rows"):
             store(qkv=behind, q_out=held[:T, 8:], **rest)
+
+
+@pytest.mark.parametrize("call, bad", (
+    (decode, dict(tables=e(2 ** 32 + 4), table_stride=2 ** 32 + 4)), (decode, dict(tables=e(2 ** 31), table_stride=2 ** 31)), (decode, dict(tables=e(2 ** 32 + 2), table_stride=1)),
+    (prefill, dict(num_seqs=2 ** 32 + 2, run_start=e(2 ** 32 + 3), seq_start=e(2 ** 32 + 2), tables=e(2 ** 34 + 8))),
+    (decode, dict(q=e(2 ** 32 + 3, NH * HD, dtype=BF), out=e(2 ** 32 + 3, NH * HD, dtype=BF), row_seq=e(2 ** 32 + 3), ctx_lens=e(2 ** 32 + 3))),
+    (prefill, dict(q=e(2 ** 32 + 3, NH * HD, dtype=BF), out=e(2 ** 32 + 3, NH * HD, dtype=BF))),
+    (store, dict(qkv=e(2 ** 32 + 3, (NH + 2 * NKV) * HD, dtype=BF), slots=e(2 ** 32 + 3))),
+    (read, dict(slots=e(2 ** 32 + 3), k=e(2 ** 32 + 3, NKV * HD, dtype=BF), v=e(2 ** 32 + 3, NKV * HD, dtype=BF))),
+    (decode, dict(nh=2 ** 32 + NH, q=e(1, (2 ** 32 + NH) * HD, dtype=BF), out=e(1, (2 ** 32 + NH) * HD, dtype=BF))),
+    (store, dict(nh=2 ** 32 + NH, qkv=e(1, (2 ** 32 + NH + 2 * NKV) * HD, dtype=BF)))))
+def test_counts_that_a_c_int_would_cut_are_refused(call, bad, monkeypatch):
+    """Numbers that end in a small one where 32 bits are kept of them: none of them reaches the library."""
+    monkeypatch.setattr(ops, "_call", lambda *args: pytest.fail(f"launched with {args}"))
+    with pytest.raises(ValueError, match="32 bits|rows of their own"):
+        call(**bad)
