@@ -2,9 +2,10 @@
 //
 // Of each token and kv head, of the key and of the value, a vector x of hd entries is kept as
 //   low = bf16(min x),  step = bf16((max x - low) / 15),  code = rint((x - low) / step) in 0..15  (0 where step is 0)
-// and stands for low + step * code: off by at most step / 2 where low and step are exact, which a vector of bfloat16 has for
-// low; rounding step moves the highest entry by up to 15 * 2^-9 of a step.  A vector with an Inf or a NaN (or whose range
-// passes the largest float) has step = NaN and reads as NaN in all its places; its codes are 0.
+// and stands for low + step * code: off by at most step / 2 from low on (rounding step to bfloat16 moves the highest entry by up to
+// 15 * 2^-8 of a step, which is less).  A vector of bfloat16 has nothing below low; one of float can, where low was rounded up, and
+// what lies there is off by up to 2^-8 |min x|, however small a step is.  A vector with an Inf or a NaN (or whose range passes the
+// largest float) has step = NaN and reads as NaN in all its places; its codes are 0.
 //
 // The cache is bytes [pages][kv heads][page / 16][16 * (hd + 8)]: tiles of 16 tokens, one behind the other, each
 //   key codes       8 * hd bytes   token t's at t * hd / 2; entry d in byte d / 2, the even one in its low half

@@ -1225,8 +1225,9 @@ _HEADS4 = (32, 64, 128, 256)
 def cache4_shape(pages, nkv, hd, block_size=16):
     """The shape of a 4-bit cache, a uint8 tensor: tiles of 16 tokens of one kv head, ``hd`` + 8 bytes a token for its key and its value.
     Each of the two is kept as 4-bit codes between its own smallest and largest entry: value = low + step * code, with low and step in
-    bfloat16 and step a fifteenth of the range, so that an entry is off by about half a step at most.  A vector that holds an Inf or a
-    NaN reads as NaN."""
+    bfloat16 and step a fifteenth of the range.  An entry of a bfloat16 row is off by half a step at most.  A float32 row's low is rounded, which
+    can leave entries below it: these are off by up to 2^-8 of the smallest entry's magnitude (of 64 entries of 1000 +- 1, more than twelve steps).
+    A vector that holds an Inf or a NaN, or whose range passes the largest float, reads as NaN."""
     _need(pages > 0 and nkv > 0 and hd in _HEADS4 and block_size > 0 and block_size % 16 == 0,
           "a 4-bit cache has pages of a multiple of 16 tokens and head_dim 32, 64, 128 or 256")
     return (pages, nkv, block_size // 16, 16 * (hd + 8))

@@ -714,3 +714,26 @@ def test_runs_in_front_of_their_sequence_see_nothing(ops):
         ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints([0, 2, 6]), ints([-2 ** 31, -2]), 2, 4, nh, nkv, hd, 0.1, window=window)
         want, tol = s.expect(q, [-1, -1, 1, 1, 1, 1], [(0, 0)] * 4 + [(0, 1), (1, 2) if window == 1 else (0, 2)], 0.1)
         near(out, want, tol)
+
+
+@pytest.mark.parametrize("dtype", (BF, F32))
+def test_how_far_a_token_is_off_with_entries_far_from_zero(ops, dtype):
+    """Half a kept step from low on (a nearest code; the highest entry, which step's rounding moves by up to 15 * 2^-8 of a step, is no further
+    off).  Below low, which float rows have where it was rounded up: low - x <= low - min x <= 2^-8 |min x|.  Reading back in 32 bits rounds once."""
+    gen = torch.Generator().manual_seed(53)
+    nkv, hd, T = 2, 64, 400
+    far = torch.where(torch.rand(T, 1, generator=gen) < 0.5, -1.0, 1.0) * torch.exp(torch.rand(T, 1, generator=gen) * 9)
+    x = (torch.randn(T, 3 * nkv * hd, generator=gen) + far).to(dtype).to(DEV)
+    cache = torch.zeros(ops.cache4_shape(25, nkv, hd, 16), dtype=torch.uint8, device=DEV)
+    ops.rope_cache4(x, nkv, nkv, hd, cache, ints(range(T)))
+    k, v = (torch.empty(T, nkv * hd, device=DEV) for _ in range(2))
+    ops.cache4_rows(cache, ints(range(T)), k, v)
+    _, ks, kl, _, vs, vl = plain.parts(cache, nkv, hd)
+    below = False
+    for got, want, step, low in ((k, x[:, nkv * hd:2 * nkv * hd], ks, kl), (v, x[:, 2 * nkv * hd:], vs, vl)):
+        a, b = got.double().view(T, nkv, hd), want.double().view(T, nkv, hd)
+        off, least = (a - b).abs(), b.amin(-1, keepdim=True).abs()
+        once = 2.0 ** -24 * a.abs()
+        assert bool((off <= torch.where(b < low[:T], 2.0 ** -8 * least, step[:T] / 2) + once).all())
+        below = below or bool((off > 2 * step[:T] + once).any())
+    assert below == (dtype == F32)
