@@ -737,3 +737,17 @@ def test_how_far_a_token_is_off_with_entries_far_from_zero(ops, dtype):
         assert bool((off <= torch.where(b < low[:T], 2.0 ** -8 * least, step[:T] / 2) + once).all())
         below = below or bool((off > 2 * step[:T] + once).any())
     assert below == (dtype == F32)
+
+
+@pytest.mark.parametrize("nh, nkv, hd, rows, dtype", ((4, 4, 32, 300, BF), (12, 12, 128, 90, F32)))
+def test_many_rows_of_short_contexts_in_workgroups_of_two_waves(ops, nh, nkv, hd, rows, dtype):
+    """1,024 workgroups and more for contexts of up to 75 tokens: two waves each, of 32 entries in bfloat16 and of 128 in float32."""
+    gen = torch.Generator().manual_seed(rows + hd)
+    lengths = torch.randint(0, 76, (rows,), generator=gen).tolist()
+    s = Sequences(ops, nh, nkv, hd, 32, lengths, gen, dtype)
+    q, out = queries(rows, nh * hd, dtype, gen), torch.full((rows, nh * hd), 9.0, dtype=dtype, device=DEV)
+    for window in (0, 33):
+        ops.attention_decode4(q, out, s.cache, s.dev_tables, s.stride, ints(range(rows)), ints(lengths), nh, nkv, hd, hd ** -0.5, 75, window=window)
+        some = list(range(0, rows, 3))
+        want, tol = s.expect(q[some], some, [(max(0, lengths[r] - window) if window else 0, lengths[r]) for r in some], hd ** -0.5)
+        near(out[some], want, tol)
