@@ -19,11 +19,12 @@
 // from -(B + 8) sum q, with the small terms of float queries before the large, and 8 step is in the bracket: sums stay nearer to what they
 // come to.)  One multiplication and addition for each score leaves the exponential's argument.
 //   sum p v = sum (p step) (B + c) - (B + 8) sum (p step) + sum p (low + 8 step)
-// where p step is what is rounded to bfloat16, as attention over the 16-bit cache rounds p: a second term would double the matrix work over
-// values for a part of the error that is less than the rounded output's own (normal keys and values, 1,000 tokens: 2.3e-3 of the output's norm,
-// 1.65e-3 if nothing but the output were rounded).  Float rows split it into three, which keep all 24 bits, as q is.  Its sum comes
-// from one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is
-// multiplied with is c - 8, as far from 0 as the values are from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
+// where p step is the operand: as a sum of bfloat16 numbers, two for single tokens (16 bits, as attention_decode keeps of p), one for runs (as
+// attention_prefill rounds p), three for float rows (which keep all 24 bits, as q does).  With normal keys and values, 1,000 tokens of 128 entries, one number
+// leaves the output off by 2.3e-3 of its norm, of which rounding the output itself is 1.65e-3, and two by 1.65e-3.  The second costs single tokens 2 to 8 %
+// (eight rows of 32,768 tokens 51.9 and 55.6 us) and would cost runs 14 to 30 (a prompt of 2,048 42.0 and 54.6 us).  The sum of p step comes from one more matrix
+// instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0 as the values are
+// from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
 //
 // m is not the largest score but one that no score passes by more than 2^6: it moves in few chunks, and only then do a row's four lanes
 // compare what they have and the sums get scaled.
@@ -70,7 +71,8 @@ __device__ __forceinline__ uint32_t codes(uint32_t word, int s, uint32_t mask) {
 __device__ __forceinline__ uint32_t pick_low(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t pick_high(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// Numbers as sums of bfloat16 ones: one for rows of bfloat16, three for float (24 bits).
+// Numbers as sums of bfloat16 ones: queries one for rows of bfloat16, three for float (24 bits); p step (NP of the kernel) so many, or two for
+// single tokens of bfloat16.
 template <class T> constexpr int kTerms = 1;
 template <> constexpr int kTerms<float> = 3;
 // Whether the sum over a key's codes starts from -(B + 8) sum q.  Bfloat16 rows of fewer than 128 entries have shorter sums and need the start's
@@ -178,7 +180,7 @@ __device__ __forceinline__ uint32_t in_vector_register(uint32_t x) {
 constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what the registers are bounded for
   return hd == 256 ? 1 : wide || rt == 2 ? 2 : hd == 128 ? 3 : 4;
 }
-template <class T, int HD, int RT, int W>
+template <class T, int HD, int RT, int W, int NP>
 __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
                                                               const int* __restrict__ tables, Rows rows, Shape sh, float* __restrict__ scratch) {
   constexpr int KS = HD / 32, C = HD / 16, NT = kTerms<T>;
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
         for (int j = 0; j < 2; ++j) s[rt][j] -= by;
       }
     }
-    u32x4 pf[RT][NT];
+    u32x4 pf[RT][NP];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float p_step[2][4];
@@ -382,14 +384,14 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
           p_step[j][i] = p * step;
         }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NP; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t two = pack(p_step[j][2 * i], p_step[j][2 * i + 1]);
             pf[rt][n][2 * j + i] = two;
-            if (n + 1 < NT) {
+            if (n + 1 < NP) {
               p_step[j][2 * i] -= bf16_bits_to_float(two & 0xFFFFu);
               p_step[j][2 * i + 1] -= bf16_bits_to_float(two >> 16);
             }
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
     for (int rt = 0; rt < RT; ++rt) {
       if constexpr (NT > 1) of_step[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int n = NT - 1; n >= 0; --n) of_step[rt] = product(ones, pf[rt][n], of_step[rt]);
+      for (int n = NP - 1; n >= 0; --n) of_step[rt] = product(ones, pf[rt][n], of_step[rt]);
     }
 #pragma unroll
     for (int d = 0; d < C; ++d) {
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int n = NT - 1; n >= 0; --n) o[rt][d] = product(vf, pf[rt][n], o[rt][d]);
+        for (int n = NP - 1; n >= 0; --n) o[rt][d] = product(vf, pf[rt][n], o[rt][d]);
       // (in 32 bits sums are not left to grow by B + 8 beyond what they come to)
       if constexpr (NT > 1) {
 #pragma unroll
@@ -676,7 +678,9 @@ int launch(const char* what, const void* q, int dtype, int q_stride, void* out, 
       T* ot = static_cast<T*>(out);
       const uint8_t* ct = static_cast<const uint8_t*>(cache);
       const auto walk = [&](auto rt, auto waves) {
-        attention4_kernel<T, HD, decltype(rt)::value, decltype(waves)::value><<<grid, decltype(waves)::value * kWave, 0, stream>>>(qt, ot, ct, tables, rows, s, scratch);
+        constexpr int RT = decltype(rt)::value, W = decltype(waves)::value, RUNS = kTerms<T>, SINGLE = std::max(RUNS, 2);
+        const auto kernel = rows.runs ? attention4_kernel<T, HD, RT, W, RUNS> : attention4_kernel<T, HD, RT, W, SINGLE>;
+        kernel<<<grid, W * kWave, 0, stream>>>(qt, ot, ct, tables, rows, s, scratch);
       };
       constexpr std::integral_constant<int, 1> one;
       constexpr std::integral_constant<int, 4> four;

@@ -751,3 +751,39 @@ def test_many_rows_of_short_contexts_in_workgroups_of_two_waves(ops, nh, nkv, hd
         some = list(range(0, rows, 3))
         want, tol = s.expect(q[some], some, [(max(0, lengths[r] - window) if window else 0, lengths[r]) for r in some], hd ** -0.5)
         near(out[some], want, tol)
+
+
+@pytest.mark.parametrize("nh, nkv, hd, rows, ctx, bound", ((8, 2, 64, 40, 200, 200), (8, 2, 128, 40, 300, 300), (4, 1, 32, 40, 700, 700), (2, 1, 256, 30, 100, 100), (8, 2, 64, 3, 3000, 3000),
+                                                           (40, 2, 64, 60, 90, 90), (64, 2, 128, 6, 900, 30000), (40, 1, 32, 1100, 40, 40), (36, 1, 64, 1100, 40, 40), (34, 1, 128, 1100, 40, 40),
+                                                           (40, 2, 32, 800, 200, 2000), (40, 2, 64, 800, 200, 2000), (40, 2, 128, 800, 200, 2000)))
+def test_single_tokens_keep_16_bits_of_their_weights(ops, nh, nkv, hd, rows, ctx, bound):
+    """Values around 0, whose weighted sums are small beside what they are sums of: the tolerance of 32-bit rows (sums over 16 + c), the output's
+    rounding, and of p step, kept in two bfloat16 numbers, 2^-8 of 2^-8, times c - 8, which is at most 8."""
+    gen = torch.Generator().manual_seed(hd + rows)
+    n = -(-ctx // 16)
+    cache = torch.zeros(ops.cache4_shape(n, nkv, hd, 16), dtype=torch.uint8, device=DEV)
+    ops.rope_cache4(torch.randn(ctx, 3 * nkv * hd, generator=gen).to(BF).to(DEV), nkv, nkv, hd, cache, ints(range(ctx)))
+    q, out = queries(rows, nh * hd, BF, gen), torch.empty(rows, nh * hd, dtype=BF, device=DEV)
+    lens = [max(2, ctx - 7 * r % ctx) for r in range(rows)]
+    ops.attention_decode4(q, out, cache, ints(range(n)), n, ints([0] * rows), ints(lens), nh, nkv, hd, hd ** -0.5, bound)
+    held = plain.parts(cache, nkv, hd)
+    some = list(range(0, rows, max(1, rows // 25)))
+    want, tol = plain.attend(q[some].double().view(-1, nh, hd), held, [torch.arange(ctx, device=DEV)] * len(some), [(0, lens[r]) for r in some], nh, nkv, hd ** -0.5, F32)
+    near(out[some], want, tol + 2.0 ** -8 * want.abs() + 2.0 ** -16 * 8 * held[4].max())
+
+
+@pytest.mark.parametrize("nh, nkv, hd", ((8, 4, 32), (8, 4, 64), (8, 4, 128), (8, 4, 256)))
+def test_many_runs_of_one_or_two_tokens(ops, nh, nkv, hd):
+    """1,200 workgroups of one tile of rows for contexts of up to 62 tokens: two waves each."""
+    gen = torch.Generator().manual_seed(hd)
+    seqs = 300
+    runs, starts = torch.randint(0, 3, (seqs,), generator=gen).tolist(), torch.randint(0, 60, (seqs,), generator=gen).tolist()
+    s = Sequences(ops, nh, nkv, hd, 16, [r + p for r, p in zip(runs, starts)], gen, BF)
+    first = np.concatenate([[0], np.cumsum(runs)])
+    T = int(first[-1])
+    q, out = queries(T, nh * hd, BF, gen), torch.full((T, nh * hd), 9.0, dtype=BF, device=DEV)
+    ops.attention_prefill4(q, out, s.cache, s.dev_tables, s.stride, ints(first), ints(starts), seqs, 2, nh, nkv, hd, hd ** -0.5, max_context=62)
+    seq, pos = [i for i, r in enumerate(runs) for _ in range(r)], [p + j for r, p in zip(runs, starts) for j in range(r)]
+    some = list(range(0, T, 5)) + [T - 1]
+    want, tol = s.expect(q[some], [seq[i] for i in some], [(0, pos[i] + 1) for i in some], hd ** -0.5)
+    near(out[some], want, tol)
