@@ -30,7 +30,7 @@
 // compare what they have and the sums get scaled.
 //
 // How the work is laid out (a rule on sizes, `plan`): the W waves of a workgroup share a tile of rows and take every W-th 32 tokens; their m, l, o
-// meet in LDS.  Single tokens are bound by reading the cache, runs of many rows by vector instructions (some 250 of a wave for 32 rows and 32
+// meet in LDS.  Single tokens are bound by reading the cache, runs of many rows by vector instructions (some 270 of a wave for 32 rows and 32
 // tokens of 128 entries, beside 38 matrix instructions).  Waves with rows of their own walk four times as long, and the last of them
 // alone: 446 us instead of 285 for portions of prompts behind contexts of 3,000 to 8,000 tokens (32 heads over 8 of 128); with operands that four such
 // waves make for one another in LDS, a quarter fewer instructions and a barrier every 64 tokens, 475 us.
@@ -583,7 +583,8 @@ static_assert(2 * kFill + 2 <= kMostSegments);
 
 // What a call with its contexts cut into `parts` takes, roughly: a round of 128 tokens (a chunk of each wave) is 0.8 us where the chip is
 // nearly empty and 2.5 where it is full; joining is a launch, the parts that a row's workgroup goes through, the workgroups, and the bytes.
-// One row, 8 kv heads of 128: 8,192 tokens take 11.0 us in 64 parts and 9.1 in 32; 2,048 tokens 7.5 us in 16 and 7.9 in 8.
+// One row, 8 kv heads of 128: 8,192 tokens take 10.9 us in 64 parts and 9.0 in 32; 2,048 tokens 7.3 us in 16 and 7.8 in 8.  (All rows count as
+// having the longest context, and all sequences the longest run: calls of unlike ones are cut less than they could be.)
 double expected_us(long long parts, long long groups, long long rounds, long long T, int nh, int hd) {
   const long long passes = (groups * parts + kFill - 1) / kFill;
   const double load = static_cast<double>(groups * parts) / (passes * kFill), walk = passes * ((rounds + parts - 1) / parts) * (0.8 + 1.7 * load);
@@ -606,9 +607,9 @@ Plan plan(bool wide, int units, int T, int max_run, int nh, int nkv, int hd, int
     rounds = (seen + LEAST - 1) / LEAST;
   };
   // Two tiles of rows to a wave share its operands; one tile leaves twice as many workgroups, and is the faster while there is work for less than
-  // two rounds of a full chip (32 heads over 8 of 128, one tile and two: four runs of 16 behind 500 tokens 7.2 us and 9.8, 16 of 64 behind 300
-  // 23.3 and 17.7; over 4 of 64: a prompt of 256 5.4 and 6.1, of 2,048 58 and 44).  Float rows, whose terms take the registers, always one (over 4 of
-  // 64, a prompt of 2,048 91 us and 94; over 8 of 128, three runs of 300 behind 4,000 211 and 276), and so 256 entries.
+  // two rounds of a full chip (32 heads over 8 of 128, one tile and two: four runs of 16 behind 500 tokens 7.2 us and 9.5, 16 of 64 behind 300
+  // 21.8 and 16.1; over 4 of 64: a prompt of 256 5.1 and 6.0, of 2,048 55 and 42).  Float rows, whose terms take the registers, always one (over 8 of
+  // 128, three runs of 300 behind 4,000 tokens 212 us and 669; over 4 of 64, a prompt of 2,048 78 and 73), and so 256 entries.
   p.waves = 4;
   tile(pairs > 16 && hd <= 128 && !wide ? 2 : 1);
   if (p.rt == 2 && groups * rounds < 2 * kFill) tile(1);
@@ -622,18 +623,18 @@ Plan plan(bool wide, int units, int T, int max_run, int nh, int nkv, int hd, int
   };
   for (long long n = 2; n <= most; n += n & (n - 1) ? n / 3 : n / 2) consider(n);
   consider(kFill / groups);
-  // Few workgroups and up to 1,024 tokens: eight waves instead of four, and no parts (32 heads over 4 of 64, one row: 529 tokens 5.7 us, with
-  // four waves 6.2; 1,000 tokens 7.4 us, in parts 6.9 and a second launch for the host).
+  // Few workgroups and up to 1,024 tokens: eight waves instead of four, and no parts (32 heads over 4 of 64, one row: 529 tokens 6.0 us, with
+  // four waves 6.7; 1,000 tokens 7.8 us, in eight parts 6.7 and a second launch for the host).
   if (p.rt == 1 && hd <= 128 && groups <= 256 && rounds > 2 && seen <= 1024) {
     parts = 1;
     p.waves = 8;
   }
   // Many workgroups of few rounds: two waves, whose beginning and end (half of a short walk) are half as many (32 heads over 8 of 128: 128 rows
-  // of 300 tokens 12.0 us, with four waves 14.8; 256 of 1,000 59.9 and 54.9.  Over 4 of 64: eight prompts of 128 tokens 7.9 us and 11.0, one of
-  // 1,024 21.1 and 17.9).
+  // of 300 tokens 11.9 us, with four waves 14.8; 256 of 1,000 60.6 and 55.0.  Over 4 of 64: eight prompts of 128 tokens 8.2 us and 10.2, one of
+  // 1,024 20.0 and 16.7).
   if (parts == 1 && groups >= 1024 && (p.rt == 1 ? 3 : 2) * seen <= groups) p.waves = 2;
-  // Of 256 entries a CU holds four waves: two workgroups where there are enough (16 heads over 2: 200 rows of 300 tokens 11.7 us, with four
-  // waves 16.4; a prompt of 2,048 91 and 108).
+  // Of 256 entries a CU holds four waves: two workgroups where there are enough (16 heads over 2: 200 rows of 300 tokens 12.0 us, with four
+  // waves 17.1; a prompt of 2,048 92 and 110).
   if (parts == 1 && groups > 256 && hd == 256) p.waves = 2;
   p.segment = parts == 1 ? LEAST : static_cast<int>(std::max<long long>(LEAST, ((seen + parts - 1) / parts + LEAST - 1) / LEAST * LEAST));
   p.max_segs = parts == 1 ? 1 : static_cast<int>((static_cast<long long>(max_context) + p.segment - 1) / p.segment);

@@ -1353,7 +1353,8 @@ def attention_decode4(q, out, cache, tables, table_stride, row_seq, ctx_lens, nh
     context of 0, a sequence without a table) gives zeros, and so would one whose pages all lie outside the cache: a table's entry that is
     no page hides its tokens.  ``max_context`` bounds every row's context length (what lies beyond it is not looked at) and decides how contexts are cut into parts that run side
     by side, which needs ``scratch`` (attention_decode4_scratch floats; allocated here when not given).  Up to 65,535 rows; keys' and values'
-    ranges up to some 1e27, beyond which sums over them overflow."""
+    ranges up to some 1e27, beyond which sums over them overflow; ``out`` is memory that no operand uses.  Scores and sums are kept in 32 bits; with
+    bfloat16 rows 16 bits are kept of what weighs a value, as in ``attention_decode``."""
     T = q.shape[0] if rows is None else rows
     q_at, out_at, cache_at, tables_at, seq_at, lens_at, scratch_at = _one_gpu(q, out, cache, tables, row_seq, ctx_lens, scratch)
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
@@ -1393,7 +1394,9 @@ def attention_prefill4(q, out, cache, tables, table_stride, run_start, seq_start
     """Causal attention over a 4-bit cache for runs of consecutive positions, as ``attention_prefill`` has them: sequence s owns rows
     run_start[s] .. run_start[s+1]-1, at most ``max_run``, the first of them at position seq_start[s]; every row sees the sequence's cached
     tokens up to its own position (``window`` > 0: the last ``window`` of them).  Rows of no run are left as they are.
-    ``max_context``: a bound of every row's context length (default: what the tables can hold).  Up to 65,535 sequences."""
+    ``max_context``: a bound of every row's context length (default: what the tables can hold).  Up to 65,535 sequences.  Ranges and ``out`` as for ``attention_decode4``;
+    with bfloat16 rows what weighs a value is rounded to bfloat16, as in ``attention_prefill``.  Every sequence is planned as if its run were ``max_run``
+    long: the single tokens of a step that has long runs beside them are better handed to ``attention_decode4``."""
     T = q.shape[0] if rows is None else rows
     q_at, out_at, cache_at, tables_at, run_at, start_at, scratch_at = _one_gpu(q, out, cache, tables, run_start, seq_start, scratch)
     pages, page = _check_cache4(cache, cache_at, nkv, hd, nh)
