@@ -22,8 +22,8 @@
 // where p step is the operand: as a sum of bfloat16 numbers, two for single tokens (16 bits, as attention_decode keeps of p), one for runs (as
 // attention_prefill rounds p), three for float rows (which keep all 24 bits, as q does).  With normal keys and values, 1,000 tokens of 128 entries, one number
 // leaves the output off by 2.3e-3 of its norm, of which rounding the output itself is 1.65e-3, and two by 1.65e-3.  The second costs single tokens 2 to 8 %
-// (eight rows of 32,768 tokens 51.9 and 55.6 us) and would cost runs 14 to 30 (a prompt of 2,048 42.0 and 54.6 us).  The sum of p step comes from one more matrix
-// instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0 as the values are
+// (eight rows of 32,768 tokens 51.9 and 55.6 us), with more than 16 heads to a kv head 4 to 15 (32 over one of 64, 1,500 rows of 400 18.4 and 21.2),
+// and would cost runs 14 to 30 (a prompt of 2,048 42.0 and 54.6 us).  The sum of p step comes from one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0 as the values are
 // from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
 //
 // m is not the largest score but one that no score passes by more than 2^6: it moves in few chunks, and only then do a row's four lanes
@@ -177,8 +177,10 @@ __device__ __forceinline__ uint32_t in_vector_register(uint32_t x) {
 
 // blockIdx.x: kv head (fastest: with eight of them each of the chip's eight parts keeps to one), then segment, then tile of rows, the last
 // tile first (it sees the most keys); blockIdx.y: token or sequence.
-constexpr int least_waves(bool wide, int hd, int rt) {      // on a SIMD: what the registers are bounded for
-  return hd == 256 ? 1 : wide || rt == 2 ? 2 : hd == 128 ? 3 : 4;
+// Waves on a SIMD that the registers are bounded for.  (Two tiles of rows and 64 entries: three, also where single tokens' second term of p step then
+// spills two or three registers: 32 heads over one, 1,500 rows of 400 tokens 21.2 us, with two waves 27.8; 2,000 of 40 12.7 and 12.0.)
+constexpr int least_waves(bool wide, int hd, int rt) {
+  return hd == 256 ? 1 : wide || (rt == 2 && hd == 128) ? 2 : rt == 2 || hd == 128 ? 3 : 4;
 }
 template <class T, int HD, int RT, int W, int NP>
 __global__ void __launch_bounds__(W * kWave, least_waves(sizeof(T) == 4, HD, RT)) attention4_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache,
