@@ -23,8 +23,9 @@
 // attention_prefill rounds p), three for float rows (which keep all 24 bits, as q does).  With normal keys and values, 1,000 tokens of 128 entries, one number
 // leaves the output off by 2.3e-3 of its norm, of which rounding the output itself is 1.65e-3, and two by 1.65e-3.  The second costs single tokens 2 to 8 %
 // (eight rows of 32,768 tokens 51.9 and 55.6 us), with more than 16 heads to a kv head 4 to 15 (32 over one of 64, 1,500 rows of 400 18.4 and 21.2),
-// and would cost runs 14 to 30 (a prompt of 2,048 42.0 and 54.6 us).  The sum of p step comes from one more matrix instruction with ones, so that B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0 as the values are
-// from their middle.  sum p and sum p (low + 8 step) stay in 32 bits.
+// and would cost runs 14 to 30 (a prompt of 2,048 42.0 and 54.6 us).  The sum of p step comes from one more matrix instruction with ones, so that
+// B + 8 cancels exactly as rounded; what the rounding is multiplied with is c - 8, as far from 0 as the values are from their middle.  sum p and
+// sum p (low + 8 step) stay in 32 bits.
 //
 // m is not the largest score but one that no score passes by more than 2^6: it moves in few chunks, and only then do a row's four lanes
 // compare what they have and the sums get scaled.
